@@ -16,7 +16,7 @@ SCALARS = {"int32_t": "i32", "uint32_t": "u32", "uint64_t": "u64", "int64_t": "i
 OPAQUE = ["runit_ctx_t", "runit_graph_t", "runit_model_t", "runit_gguf_t"]
 STRUCTS = ["runit_model_cfg", "runit_model_weights", "runit_sampler_cfg", "runit_gguf_tensor_info",
            "runit_layer_desc", "runit_layered_cfg", "runit_layered_weights", "runit_latent_cfg",
-           "runit_heads_cfg", "runit_retention_cfg", "runit_ssm_cfg", "runit_linear_cfg"]
+           "runit_heads_cfg", "runit_retention_cfg", "runit_ssm_cfg", "runit_linear_cfg", "runit_paged_cfg", "runit_paged_batch"]
 # operators that are not GPU ops of the dispatch layer (context, buffers, recording): wrapped by hand in context.rs
 NOT_OPS = {"runit_ctx_create", "runit_ctx_create_on_stream", "runit_ctx_destroy", "runit_flush", "runit_buf_alloc", "runit_buf_free",
            "runit_memcpy_h2d", "runit_memcpy_d2h", "runit_memset", "runit_set_tuning", "runit_graph_begin", "runit_graph_end",
@@ -123,6 +123,12 @@ def gen():
             "    pub heads: u32, pub groups: u32, pub dk: u32, pub dv: u32, pub ldq: u32, pub ldk: u32, pub ldv: u32, pub ldo: u32,",
             "    pub q: *const c_void, pub k: *const c_void, pub v: *const c_void, pub dt: *const c_void, pub log_decay: *const c_void,",
             "    pub decay: *const c_void, pub skip: *const c_void, pub state: *mut c_void, pub out: *mut c_void,", "}",
+            "#[repr(C)]", "#[derive(Clone, Copy, Debug)]", "pub struct runit_paged_cfg {",
+            "    pub heads: u32, pub kv_heads: u32, pub dim: u32, pub page: u32, pub n_pages: u32, pub type_: i32, pub window: u32,",
+            "    pub scale: f32, pub cap: f32, pub slopes: *const c_void, pub k_pages: *mut c_void, pub v_pages: *mut c_void,", "}",
+            "#[repr(C)]", "#[derive(Clone, Copy, Debug)]", "pub struct runit_paged_batch {",
+            "    pub n_seqs: u32, pub rows: u32, pub table_ld: u32, pub shared_len: u32,",
+            "    pub table: *const c_void, pub q_start: *const c_void, pub kv_len: *const c_void,", "}",
             "#[repr(C)]", "#[derive(Clone, Copy, Debug)]", "pub struct runit_layered_cfg {",
             "    pub n_layers: i32, pub width: i32, pub vocab: i32, pub max_seq: i32, pub exact: i32, pub post_norm: i32,",
             "    pub eps: f32, pub embed_scale: f32, pub logit_cap: f32,", "}",

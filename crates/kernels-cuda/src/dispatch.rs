@@ -254,6 +254,9 @@ pub fn gemv_bf16_residual_f32(ctx: &CudaContext, weight: &B, x: &B, y: &B, y_gai
 pub fn gemv_bf16_groups_f32(ctx: &CudaContext, weight: &B, x: &B, factor: &B, squares: &B, squares_n: u32, out: &B, eps: f32, plain: u32, group: u32, m: u32, k: u32) -> Result<()> {
     ctx.check(unsafe { ffi::runit_gemv_bf16_groups_f32(ctx.raw, weight.ptr as *const c_void, x.ptr as *const c_void, factor.ptr as *const c_void, squares.ptr as *const c_void, squares_n, out.ptr, eps, plain, group, m, k) })
 }
+pub fn token_logprobs(ctx: &CudaContext, logits: &B, r#type: i32, ld: u32, n: u32, rows: u32, tokens: &B, logprob: &B, entropy: &B, k: u32, top_ids: &B, top_logprobs: &B) -> Result<()> {
+    ctx.check(unsafe { ffi::runit_token_logprobs(ctx.raw, logits.ptr as *const c_void, r#type, ld, n, rows, tokens.ptr as *const c_void, logprob.ptr, entropy.ptr, k, top_ids.ptr, top_logprobs.ptr) })
+}
 pub fn fill_weights(ctx: &CudaContext, fmt: i32, dst: &B, n_blocks: u64, seed: u64, sigma: f32) -> Result<()> {
     ctx.check(unsafe { ffi::runit_fill_weights(ctx.raw, fmt, dst.ptr, n_blocks, seed, sigma) })
 }

@@ -98,6 +98,18 @@ pub struct runit_linear_cfg {
 }
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
+pub struct runit_paged_cfg {
+    pub heads: u32, pub kv_heads: u32, pub dim: u32, pub page: u32, pub n_pages: u32, pub type_: i32, pub window: u32,
+    pub scale: f32, pub cap: f32, pub slopes: *const c_void, pub k_pages: *mut c_void, pub v_pages: *mut c_void,
+}
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct runit_paged_batch {
+    pub n_seqs: u32, pub rows: u32, pub table_ld: u32, pub shared_len: u32,
+    pub table: *const c_void, pub q_start: *const c_void, pub kv_len: *const c_void,
+}
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
 pub struct runit_layered_cfg {
     pub n_layers: i32, pub width: i32, pub vocab: i32, pub max_seq: i32, pub exact: i32, pub post_norm: i32,
     pub eps: f32, pub embed_scale: f32, pub logit_cap: f32,
@@ -251,6 +263,10 @@ extern "C" {
     pub fn runit_add_norm_rows(a0: *mut runit_ctx_t, x: *mut c_void, y: *const c_void, gain: *const c_void, eps: f32, out_gain: *const c_void, out: *mut c_void, out_f32: i32, T: u32, width: u32) -> i32;
     pub fn runit_gemv_bf16_residual_f32(a0: *mut runit_ctx_t, weight: *const c_void, x: *const c_void, y: *const c_void, y_gain: *const c_void, gain: *const c_void, x_out: *mut c_void, out: *mut c_void, eps: f32, cap: f32, relu2: i32, m: u32, k: u32) -> i32;
     pub fn runit_gemv_bf16_groups_f32(a0: *mut runit_ctx_t, weight: *const c_void, x: *const c_void, factor: *const c_void, squares: *const c_void, squares_n: u32, out: *mut c_void, eps: f32, plain: u32, group: u32, m: u32, k: u32) -> i32;
+    pub fn runit_paged_append(a0: *mut runit_ctx_t, cfg: *const runit_paged_cfg, batch: *const runit_paged_batch, proj: *const c_void, proj_type: i32, ld: u32, freq: *const c_void, rot_dims: u32, q_out: *mut c_void, ldq: u32) -> i32;
+    pub fn runit_paged_attention_scratch_bytes(cfg: *const runit_paged_cfg, batch: *const runit_paged_batch) -> usize;
+    pub fn runit_paged_attention(a0: *mut runit_ctx_t, cfg: *const runit_paged_cfg, batch: *const runit_paged_batch, q: *const c_void, ldq: u32, out: *mut c_void, ldo: u32, scratch: *mut c_void, scratch_bytes: usize) -> i32;
+    pub fn runit_token_logprobs(a0: *mut runit_ctx_t, logits: *const c_void, r#type: i32, ld: u32, n: u32, rows: u32, tokens: *const c_void, logprob: *mut c_void, entropy: *mut c_void, k: u32, top_ids: *mut c_void, top_logprobs: *mut c_void) -> i32;
     pub fn runit_model_create_layered(ctx: *mut runit_ctx_t, cfg: *const runit_layered_cfg, layers: *const runit_layer_desc, weights: *const runit_layered_weights, out: *mut *mut runit_model_t) -> i32;
     pub fn runit_model_residual(model: *mut runit_model_t) -> *mut c_void;
     pub fn runit_model_set_depth(model: *mut runit_model_t, n_layers: i32) -> i32;

@@ -614,6 +614,51 @@ int32_t runit_gemv_bf16_residual_f32(runit_ctx_t*, const void* weight, const voi
 int32_t runit_gemv_bf16_groups_f32(runit_ctx_t*, const void* weight, const void* x, const void* factor, const void* squares, uint32_t squares_n,
                                    void* out, float eps, uint32_t plain, uint32_t group, uint32_t m, uint32_t k);
 
+/* ── serving a batch of sequences over a paged cache of keys and values (no twin: the reference caches one sequence) ──
+ * Pages of `page` positions (a power of two, 16 to 256), f16 or bf16: k_pages, v_pages [n_pages][kv_heads][page][dim], 128-byte aligned.  Query head
+ * h uses key head h / (heads / kv_heads); dim 64 or 128.  Position p of sequence s lies in row p % page of page table[s][p / page]; table entries
+ * behind a sequence's last page are not read.  Sequence s has rows q_start[s] .. q_start[s + 1] - 1 of the tensors, which are its last positions
+ * (kv_len[s] counts the positions, those of its rows included); rows from q_start[n_seqs] on belong to nobody and are left as they are.
+ * table, q_start and kv_len are device memory, so that a recorded list serves other lengths: a page outside the pool, a length that the table does
+ * not hold or that is shorter than the sequence's rows makes the next flush return RUNIT_ERR_BAD_ARG; nothing outside the tensors is touched. */
+enum { RUNIT_TYPE_F32 = 0, RUNIT_TYPE_F16 = 1, RUNIT_TYPE_BF16 = 2 };
+typedef struct {
+    uint32_t heads, kv_heads, dim, page, n_pages;
+    int32_t  type;           /* of the cache, RUNIT_TYPE_F16 or RUNIT_TYPE_BF16 */
+    uint32_t window;         /* 0: all earlier positions, else a position sees itself and the window - 1 before it */
+    float    scale, cap;     /* scores (q . k) * scale; cap != 0: then cap * tanh(score / cap) */
+    const void* slopes;      /* f32 [heads]: score - slopes[h] * (i - j) for query position i and key position j; NULL: no bias */
+    void*    k_pages;
+    void*    v_pages;
+} runit_paged_cfg;
+typedef struct {
+    uint32_t n_seqs, rows, table_ld;   /* n_seqs up to 4096; rows: of the tensors; table rows of table_ld pages */
+    uint32_t shared_len;     /* a multiple of `page`: the first shared_len positions are the same for all sequences and lie in the pages of table row 0 */
+    const void* table;       /* int32 [n_seqs][table_ld] */
+    const void* q_start;     /* int32 [n_seqs + 1], ascending from 0, the last one at most `rows` */
+    const void* kv_len;      /* int32 [n_seqs] */
+} runit_paged_batch;
+/* Projected rows [q: heads x dim | k, v: kv_heads x dim] of ld elements (proj_type f32 or the cache's type): the first rot_dims coordinates of q and
+ * k are rotated (pairs (i, i + rot_dims / 2), angle position * (freq[0][i] + freq[1][i]), freq f32 [2][rot_dims / 2] as for the retention; rot_dims
+ * 0: none), k and v go to the pages of their positions, q to q_out (rows of ldq elements of the cache's type; NULL: keys and values only).  f32
+ * arithmetic, rounded once.  A page that gets rows belongs to one sequence. */
+int32_t runit_paged_append(runit_ctx_t*, const runit_paged_cfg* cfg, const runit_paged_batch* batch, const void* proj, int32_t proj_type, uint32_t ld,
+                           const void* freq, uint32_t rot_dims, void* q_out, uint32_t ldq);
+/* out[row][head] = softmax over the positions that the row sees (those up to its own, within the window) of its scores, times their values.  q and out:
+ * the cache's type, rows of ldq / ldo elements (multiples of 8), 16-byte aligned.  Scores, softmax and sums are f32; the weights are rounded to the cache's
+ * type where they meet the values.  The shared positions are read once for all sequences.  A row that sees nothing gets zeros.  Values of positions that
+ * a row does not see do not reach it, whatever they are.  scratch: 256-byte aligned, runit_paged_attention_scratch_bytes of it (which no two calls
+ * in flight may share; it depends on the sizes in cfg and batch alone and needs no clearing). */
+size_t  runit_paged_attention_scratch_bytes(const runit_paged_cfg* cfg, const runit_paged_batch* batch);   /* 0: a description that the call refuses */
+int32_t runit_paged_attention(runit_ctx_t*, const runit_paged_cfg* cfg, const runit_paged_batch* batch, const void* q, uint32_t ldq, void* out,
+                              uint32_t ldo, void* scratch, size_t scratch_bytes);
+/* Rows of n logits (type f32, f16 or bf16; ld elements apart): logprob f32 [rows] = log softmax at tokens[row] (int32; 0 for a token outside 0 .. n - 1,
+ * which marks a row without one; tokens and logprob may both be NULL), entropy f32 [rows] of the softmax (may be NULL), and its k most probable entries
+ * (k <= 32 and k <= n): top_ids int32 [rows][k], descending, equal logits by index, and top_logprobs f32 [rows][k] (both NULL with k = 0).  A NaN counts as
+ * the largest logit and makes the row's values NaN; in a row of -Inf alone every log probability is -Inf and the entropy 0. */
+int32_t runit_token_logprobs(runit_ctx_t*, const void* logits, int32_t type, uint32_t ld, uint32_t n, uint32_t rows, const void* tokens, void* logprob,
+                             void* entropy, uint32_t k, void* top_ids, void* top_logprobs);
+
 /* ── decoders described layer by layer (no twin), weights in bf16 ──
  * Every matrix is row-major [rows][pad8(columns)] bf16 with zero padding; norms and router are f32.  Linear maps W x.
  * Residual stream, norms, scores, softmax, router, angles and recurrent state are f32.  norm(x) = x / sqrt(mean(x^2) + eps) * gain.

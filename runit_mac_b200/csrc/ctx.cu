@@ -210,6 +210,9 @@ int32_t runit_flush(runit_ctx_t* ctx) {
         if (why == 4) {
             runit_fail(ctx, RUNIT_ERR_UNSUPPORTED, "sampler: top-k is off and the nucleus is wider than the 1024 most probable tokens (code %d)", why);
             if (ctx->sticky_status == RUNIT_OK) ctx->sticky_status = RUNIT_ERR_UNSUPPORTED;   // reported by this flush
+        } else if (why == 5) {
+            runit_fail(ctx, RUNIT_ERR_BAD_ARG, "paged cache: a page outside the pool, or a length that the table or the sequence's rows contradict (code %d)", why);
+            if (ctx->sticky_status == RUNIT_OK) ctx->sticky_status = RUNIT_ERR_BAD_ARG;
         } else
         runit_fail(ctx, RUNIT_ERR_TIMEOUT, why == 3 ? "a peer barrier gave up: a rank never announced its epoch (code %d)"
                                                     : "a kernel gave up a bounded wait (a copy or a dependency never completed; code %d)", why);

@@ -96,7 +96,7 @@ def _ptr(b) -> int:
 
 # What an argument of a call becomes, by its type: nothing here looks at a value, and a type of buffers is entered when it is first seen.  (Asking every
 # argument whether it is a buffer took 2.6 of the 6.0 us of a small GEMV's call.)
-_CONVERT = {DeviceBuffer: lambda b: b.ptr, float: float, type(None): lambda n: None}
+_CONVERT = {DeviceBuffer: lambda b: b.ptr, float: float, type(None): lambda n: None, type(C.byref(C.c_int32())): lambda r: r}
 
 
 def _convert(a):
@@ -320,6 +320,9 @@ _TWINS = [
     ("add_norm_rows", "no twin: (x, y or None, gain, eps, out_gain or None, out or None, out_f32, T, width)"),
     ("gemv_bf16_residual_f32", "no twin: (weight, x, y or None, y_gain, gain or None, x_out or None, out, eps, cap, relu2, m, k)"),
     ("gemv_bf16_groups_f32", "no twin: (weight, x, factor, squares or None, squares_n, out, eps, plain, group, m, k)"),
+    ("paged_append", "no twin: (PagedCfg ref, PagedBatch ref, proj, proj_type, ld, freq or None, rot_dims, q_out or None, ldq)"),
+    ("paged_attention", "no twin: (PagedCfg ref, PagedBatch ref, q, ldq, out, ldo, scratch, scratch_bytes)"),
+    ("token_logprobs", "no twin: (logits, type, ld, n, rows, tokens or None, logprob or None, entropy or None, k, top_ids or None, top_logprobs or None)"),
     ("fill_weights", "no twin: (fmt, dst, n_blocks, seed, sigma)"),
     ("fill_weights_q4k_zero_mean", "no twin: (dst, n_blocks, seed, sigma), Q4_K blocks with zero-mean weights"),
     ("fill_normal_f32", "no twin: (dst, n, seed, sigma)"),
@@ -486,6 +489,20 @@ class LinearCfg(C.Structure):
                 [(n, C.c_void_p) for n in ("q", "k", "v", "dt", "log_decay", "decay", "skip", "state", "out")])
 
 
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+
+
+class PagedCfg(C.Structure):
+    """runit_paged_cfg: the paged cache of a layer and its scores; pass ``ctypes.byref(cfg)``."""
+    _fields_ = ([(n, C.c_uint32) for n in ("heads", "kv_heads", "dim", "page", "n_pages")] + [("type", C.c_int32), ("window", C.c_uint32)] +
+                [(n, C.c_float) for n in ("scale", "cap")] + [(n, C.c_void_p) for n in ("slopes", "k_pages", "v_pages")])
+
+
+class PagedBatch(C.Structure):
+    """runit_paged_batch: rows, lengths and pages of the sequences of a step; pass ``ctypes.byref(batch)``."""
+    _fields_ = ([(n, C.c_uint32) for n in ("n_seqs", "rows", "table_ld", "shared_len")] + [(n, C.c_void_p) for n in ("table", "q_start", "kv_len")])
+
+
 class LayerDesc(C.Structure):
     """runit_layer_desc: mixer and feed-forward of one layer, sizes, constants and device pointers."""
     _fields_ = ([(n, C.c_int32) for n in ("heads", "dim", "rot_dim", "vdim", "kv_rank", "kv_from")] +
@@ -544,6 +561,11 @@ def moe_grouped_scratch_bytes(ctx: Context, T: int, h: int, ff: int, E: int, k: 
     return ctx.lib.runit_moe_grouped_scratch_bytes(T, h, ff, E, k)
 
 
+def paged_attention_scratch_bytes(ctx: Context, cfg: PagedCfg, batch: PagedBatch) -> int:
+    """0 for a description that paged_attention refuses."""
+    return ctx.lib.runit_paged_attention_scratch_bytes(C.byref(cfg), C.byref(batch))
+
+
 def moe_layer_q4k_bf16_host(ctx: Context, router, gate, up, down, x, *, h, ff, E, top_k, renorm=False, residual=None,
                             routing=None):
     """Convenience for tests: upload host arrays, run the batched tensor-core block once, download
@@ -584,6 +606,6 @@ def moe_layer_q4k_host(ctx: Context, router, gate, up, down, x, *, h, ff, E, top
             w.download(np.float32, T * top_k).reshape(T, top_k))
 
 
-__all__ = ["Context", "DeviceBuffer", "Graph", "KernelError", "Model", "ModelCfg", "ModelWeights", "LayeredModel", "LayeredCfg", "LayeredWeights", "LayerDesc", "LatentCfg", "HeadsCfg", "RetentionCfg", "SsmCfg", "LinearCfg", "EPI_F32", "EPI_ADD", "EPI_CAST", "EPI_SILU_GLU", "EPI_RELU2",
+__all__ = ["Context", "DeviceBuffer", "Graph", "KernelError", "Model", "ModelCfg", "ModelWeights", "LayeredModel", "LayeredCfg", "LayeredWeights", "LayerDesc", "LatentCfg", "HeadsCfg", "RetentionCfg", "SsmCfg", "LinearCfg", "PagedCfg", "PagedBatch", "TYPE_F32", "TYPE_F16", "TYPE_BF16", "paged_attention_scratch_bytes", "EPI_F32", "EPI_ADD", "EPI_CAST", "EPI_SILU_GLU", "EPI_RELU2",
            "FF_NONE", "FF_DENSE", "FF_MOE", "MIX_LATENT", "MIX_HEADS", "MIX_SSM", "ACT_SILU_GLU", "ACT_RELU2", "SCORE_SOFTMAX", "SCORE_SIGMOID", "SamplerCfg", "sample_f32", "sampler_seed_state", "gemv_batched_multi_f32", "moe_scratch_bytes", "moe_layer_q4k_host", "moe_grouped_scratch_bytes", "moe_layer_q4k_bf16_host", "row_bytes", "BLOCK_ELEMS", "BLOCK_BYTES",
            "FMT_Q8_0", "FMT_Q4_0", "FMT_Q4K", "FMT_Q5_0", "FMT_Q5K", "FMT_Q6K"] + [n for n, _ in _TWINS]
