@@ -67,6 +67,9 @@ static inline const char* why_not(const runit_paged_cfg* g, const runit_paged_ba
     if (b->rows == 0 || (uint64_t)b->rows * g->heads > 0x7FFFFFFFull) return "rows must not be 0, and rows * heads below 2^31";
     if (b->table_ld == 0 || (uint64_t)b->table_ld * g->page > 0x7FFFFFFFull) return "table_ld must not be 0, and table_ld * page below 2^31";
     if (b->shared_len % g->page != 0 || b->shared_len / g->page > b->table_ld) return "shared_len must be whole pages, as many as a table row has at most";
+    // steps of 16 positions and 16 (row, query head) pairs of a key head, all sequences together, are counted in 32 bits
+    const uint64_t tiles = (uint64_t)b->rows * (g->heads / g->kv_heads) / 16 + b->n_seqs + 1, steps = (uint64_t)b->table_ld * g->page / 16 + 1;
+    if (tiles * g->kv_heads >= 1ull << 32 || tiles * g->kv_heads * steps >= 1ull << 32) return "rows, sequences and table_ld * page are too many together";
     return nullptr;
 }
 static inline const char* why_not_memory(const runit_paged_cfg* g, const runit_paged_batch* b) {

@@ -1,71 +1,599 @@
 // Attention of a batch of sequences over a paged cache: out_i = sum_j softmax_j(s_ij) v_j over the positions j that row i sees, s_ij = scale q_i . k_j,
 // then cap * tanh(s / cap), then minus slope * (i - j).
-#include "gemv_common.cuh"
-#include "paged.cuh"
-#include "tma.cuh"
+//
+// Few rows a sequence (decoding): bound by HBM, which has to deliver every key and value once.  A segment is what shares keys: up to 16 (row, query head)
+// pairs of one sequence and key head, and the positions that they see; the segments' steps of 32 positions, one behind the other, are dealt out evenly to
+// the warps of the grid, whatever the lengths.  A warp is on its own: it copies its steps by TMA into a ring (boxes of 16 positions, so that pages of
+// 16 are whole boxes), multiplies on the legacy tensor path with the rows as m16 (a tcgen05 tile would be 128 rows, mostly padding), and keeps
+// maximum, sum and output of the running softmax in registers.  Segments that a warp has whole are done with that; the others leave a piece per warp, and
+// merge_kernel adds them up.
+#include "paged_attention.cuh"
 
 namespace runit {
 namespace pg {
 
-struct AttnArgs {
-    Cache c;
-    const void* q;
-    void* out;
-    const float* slopes;
-    uint32_t ldq, ldo, window;
-    float scale, cap;
+constexpr uint32_t kWarps = 4, kStep = 32, kBox = 16, kRows = 16, kPlanHead = 16;
+constexpr uint32_t kMaxWorkers = kWarps * 256;
+constexpr uint32_t kStepsMin = 2;              // a worker's share at least: what it costs to begin and to merge is that of about two steps
+
+template <int HD> struct Shape {
+    static constexpr uint32_t kBoxBytes = kBox * HD * 2, kStage = 4 * kBoxBytes, kStages = HD == 128 ? 3 : 6;
+    static constexpr uint32_t kRing = kStage * kStages * kWarps;
 };
 
-// The plainest form: a block per row and query head, four warps that take its keys in turn, a lane 2 or 4 of the dimensions.
+// ── segments ──
+// Entry e < n_seqs: a sequence and its own positions (from c.shared on); entry n_seqs (with shared positions): all rows and the shared ones.
+struct Entry {
+    uint32_t row0, n, tiles, lo, hi, steps;    // steps of one (key head, tile): the positions lo (down to a box) .. hi that any row of it sees
+    int32_t base;                              // position of its first row
+    const int32_t* table;
+};
+__device__ __forceinline__ uint32_t steps_of(uint32_t lo, uint32_t hi) { return hi > lo ? (hi - (lo & ~(kBox - 1)) + kStep - 1) / kStep : 0; }
+__device__ __forceinline__ Entry entry_of(const AttnArgs& a, uint32_t e, uint32_t pre_lo, uint32_t pre_hi) {
+    const Cache& c = a.c;
+    Entry t;
+    if (e < c.n_seqs) {
+        const Seq s = sequence(c, e);
+        t.row0 = s.row0;
+        t.n = s.n;
+        t.base = (int32_t)s.len - (int32_t)s.n;
+        t.lo = max(c.shared, first_seen(t.base, a.window));
+        t.hi = s.n ? s.len : 0;
+        t.table = c.table + (size_t)e * c.table_ld;
+    } else {
+        t.row0 = 0;
+        t.n = c.rows;
+        t.base = 0;
+        t.lo = pre_lo;
+        t.hi = pre_hi;
+        t.table = c.table;
+    }
+    t.tiles = (t.n * c.group + kRows - 1) / kRows;
+    t.steps = steps_of(t.lo, t.hi);
+    return t;
+}
+// Worker w of `workers` has the steps from begin_of(w) to begin_of(w + 1).
+__device__ __forceinline__ uint32_t begin_of(uint32_t w, uint32_t total, uint32_t workers) { return (uint32_t)((uint64_t)w * total / workers); }
+__device__ __forceinline__ uint32_t owner_of(uint32_t step, uint32_t total, uint32_t workers) { return (uint32_t)((((uint64_t)step + 1) * workers - 1) / total); }
+__device__ __forceinline__ uint32_t workers_of(uint32_t total, uint32_t most) { return max(1u, min(most, total / kStepsMin)); }
+
+struct Piece {
+    float *o, *ml;
+};
+__device__ __forceinline__ Piece slot_of(const AttnArgs& a, uint32_t w, bool first) {
+    const size_t s = 2 * (size_t)w + (first ? 0 : 1);
+    return Piece{a.slot_o + s * kRows * a.c.dim, a.slot_ml + s * kRows * 2};
+}
+
+// ── operations on scores ──
+struct Scoring {
+    float mul, cap, inv_cap, slope0, slope1;   // mul: scale (times log2 e without cap and bias); slopes of a thread's two rows
+    bool plain;
+};
+// A score in units of log2: x[row][key].
+__device__ __forceinline__ float score(const Scoring& s, float dot, float slope, float back) {
+    if (s.plain) return dot * s.mul;
+    float t = dot * s.mul;
+    if (s.cap != 0.f) t = s.cap * tanhf(t * s.inv_cap);
+    return (t - slope * back) * kLog2e;
+}
+
+// V of a step whose hidden positions hold something that is no number: its elements were left out of the products (0 there), the rows that see
+// them get them here.  p: the weights as the products' accumulators hold them.
 template <typename T, int HD>
-__global__ void __launch_bounds__(128) paged_attention_kernel(const AttnArgs a) {
+__device__ __noinline__ void add_not_finite(const uint8_t* stage_v, uint32_t k0, uint32_t end, const uint32_t (&lo)[2], const uint32_t (&hi)[2], const float (&p)[kStep / 8][4],
+                                            float (&o)[HD / 8][4]) {
+    const uint32_t lane = threadIdx.x & 31, t = lane & 3;
+#pragma unroll 1
+    for (uint32_t j = 0; j < kStep; j++) {
+        const uint32_t key = k0 + j;
+        if (key >= end) break;                 // nothing behind that was copied
+        float w[2] = {0.f, 0.f};
+#pragma unroll
+        for (uint32_t n = 0; n < kStep / 8; n++)
+#pragma unroll
+            for (uint32_t e = 0; e < 2; e++) {
+                const float x = __shfl_sync(0xffffffffu, p[n][e], (lane & ~3u) | ((j & 7) >> 1)), y = __shfl_sync(0xffffffffu, p[n][2 + e], (lane & ~3u) | ((j & 7) >> 1));
+                if (n == j / 8 && e == (j & 1)) { w[0] = x; w[1] = y; }
+            }
+        const uint32_t row = j % kBox;
+        const uint8_t* box = stage_v + (j / kBox) * Shape<HD>::kBoxBytes;
+#pragma unroll
+        for (uint32_t d = 0; d < HD / 8; d++) {
+            const uint32_t word = *reinterpret_cast<const uint32_t*>(box + (d >> 3) * (kBox * 128) + row * 128 + (((d & 7) ^ (row & 7)) << 4) + 4 * t);
+            const uint32_t nf = Half2<T>::not_finite(word);
+            if (!nf) continue;
+            const float2 v = Half2<T>::unpack(word);
+#pragma unroll
+            for (uint32_t r = 0; r < 2; r++) {
+                if (key < lo[r] || key >= hi[r]) continue;
+                if (nf & 0x8000u) o[d][2 * r] += w[r] * v.x;
+                if (nf & 0x80000000u) o[d][2 * r + 1] += w[r] * v.y;
+            }
+        }
+    }
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const AttnArgs a,
+                                                                   const uint32_t n_entries) {
+    using S = Shape<HD>;
+    constexpr uint32_t KS = HD / 16, ND = HD / 8, NK = kStep / 8;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[kWarps * S::kStages];
+    __shared__ uint32_t sums[kWarps], edge[2];
+    uint8_t* const ring = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
+    uint32_t* const before = reinterpret_cast<uint32_t*>(ring + S::kRing);         // [n_entries + 1] steps in front of an entry
+    const Cache& c = a.c;
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g4 = lane >> 2, t4 = lane & 3;
+    if (tid < kWarps * S::kStages) mbar_init(smem_u32(&bars[tid]), 1);
+    if (tid == 0) {
+        edge[0] = c.shared;
+        edge[1] = 0;
+    }
+    fence_mbar_init();
+    __syncthreads();
     grid_dependency_wait();
     grid_launch_dependents();
-    constexpr int E = HD / 32;
-    __shared__ float sm[4], sl[4], so[4][HD];
-    const Cache& c = a.c;
-    const uint32_t row = blockIdx.x, head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint32_t s = 0;
-    for (uint32_t i0 = 1; i0 <= c.n_seqs; i0 += 128) {
-        const uint32_t i = i0 + threadIdx.x;
-        s += __syncthreads_count(i <= c.n_seqs && c.q_start[i] <= (int32_t)row);
-    }
-    if (s >= c.n_seqs) return;
-    const Seq q = sequence(c, s);
-    const uint32_t back = q.row0 + q.n - row;
-    if (row < q.row0 || back > q.n) return;
-    const uint32_t end = q.len >= back ? q.len - back + 1 : 0, beg = a.window && end > a.window ? end - a.window : 0;
-    const T* qp = reinterpret_cast<const T*>(a.q) + (size_t)row * a.ldq + (size_t)head * HD + lane * E;
-    float x[E], o[E], m = -INFINITY, l = 0.f;
-    for (int e = 0; e < E; e++) { x[e] = to_f32(qp[e]); o[e] = 0.f; }
-    const float slope = a.slopes ? a.slopes[head] : 0.f;
-    for (uint32_t j = beg + warp; j < end; j += 4) {
-        bool ok;
-        const size_t at = page_row(c, c.table + (j < c.shared ? 0 : (size_t)s * c.table_ld), j, head / c.group, &ok) + lane * E;
-        float t = 0.f;
-        for (int e = 0; e < E; e++) t = fmaf(x[e], to_f32(reinterpret_cast<const T*>(c.k)[at + e]), t);
-        for (int d = 16; d > 0; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
-        t *= a.scale;
-        if (a.cap != 0.f) t = a.cap * tanhf(t / a.cap);
-        t -= slope * (float)(end - 1 - j);
-        const float top = fmaxf(m, t), old = m == -INFINITY ? 0.f : expf(m - top), p = expf(t - top);
-        l = fmaf(l, old, p);
-        for (int e = 0; e < E; e++) o[e] = fmaf(o[e], old, p * to_f32(reinterpret_cast<const T*>(c.v)[at + e]));
-        m = top;
-    }
-    if (lane == 0) { sm[warp] = m; sl[warp] = l; }
-    for (int e = 0; e < E; e++) so[warp][lane * E + e] = o[e];
-    __syncthreads();
-    if (threadIdx.x < HD) {
-        const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-        float num = 0.f, den = 0.f;
-        for (int w = 0; w < 4; w++) {
-            const float f = sm[w] == -INFINITY ? 0.f : expf(sm[w] - top);
-            num = fmaf(f, so[w][threadIdx.x], num);
-            den = fmaf(f, sl[w], den);
+    // the shared positions that some row sees
+    if (n_entries > c.n_seqs) {
+        uint32_t lo = c.shared, hi = 0;
+        for (uint32_t e = tid; e < c.n_seqs; e += kWarps * 32) {
+            const Seq s = sequence(c, e);
+            if (!s.n) continue;
+            lo = min(lo, first_seen((int32_t)s.len - (int32_t)s.n, a.window));
+            hi = max(hi, min(s.len, c.shared));
         }
-        reinterpret_cast<T*>(a.out)[(size_t)row * a.ldo + (size_t)head * HD + threadIdx.x] = from_f32<T>(den == 0.f ? 0.f : num / den);
+        atomicMin(&edge[0], lo);
+        atomicMax(&edge[1], hi);
+        __syncthreads();
     }
+    const uint32_t pre_lo = edge[0], pre_hi = edge[1];
+    {
+        const uint32_t per = (n_entries + kWarps * 32 - 1) / (kWarps * 32), beg = min(n_entries, tid * per), end = min(n_entries, beg + per);
+        uint32_t sum = 0;
+        for (uint32_t e = beg; e < end; e++) {
+            const Entry t = entry_of(a, e, pre_lo, pre_hi);
+            before[e] = sum;
+            sum += t.tiles * t.steps * c.kv_heads;
+        }
+        uint32_t inc = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= (uint32_t)o) inc += v;
+        }
+        if (lane == 31) sums[warp] = inc;
+        __syncthreads();
+        uint32_t off = inc - sum;
+        for (uint32_t w = 0; w < warp; w++) off += sums[w];
+        for (uint32_t e = beg; e < end; e++) before[e] += off;
+        if (tid == kWarps * 32 - 1) before[n_entries] = off + sum;
+        __syncthreads();
+    }
+    const uint32_t total = before[n_entries], workers = workers_of(total, gridDim.x * kWarps);
+    if (blockIdx.x == 0) {
+        for (uint32_t e = tid; e <= n_entries; e += kWarps * 32) a.plan[kPlanHead + e] = before[e];
+        if (tid == 0) {
+            a.plan[0] = pre_lo;
+            a.plan[1] = pre_hi;
+            a.plan[2] = workers;
+        }
+    }
+    const uint32_t me = warp * gridDim.x + blockIdx.x;          // neighbours in the order of steps sit on other SMs: few steps spread over all of them
+    if (me >= workers || total == 0) return;
+    const uint32_t x0 = begin_of(me, total, workers), x1 = begin_of(me + 1, total, workers);
+
+    // A place in the order of steps.  Reader and copier walk it, the copier kStages ahead.
+    struct Cursor {
+        Entry t;
+        uint32_t e, h, tile, lo, hi, step;     // lo, hi: positions that the tile's rows see
+    };
+    auto enter = [&](Cursor& u) {              // (e, h, tile) are set
+        u.lo = u.t.lo;
+        u.hi = u.t.hi;
+        if (u.e < c.n_seqs && u.t.tiles > 1) {
+            const uint32_t last = min(u.t.n * c.group, (u.tile + 1) * kRows) - 1;
+            const int32_t p0 = u.t.base + (int32_t)(u.tile * kRows / c.group), p1 = u.t.base + (int32_t)(last / c.group);
+            u.hi = (uint32_t)max(0, p1 + 1);
+            u.lo = max(u.lo, first_seen(p0, a.window));
+        }
+    };
+    auto seek = [&](Cursor& u, uint32_t x) {
+        uint32_t l = 0, r = n_entries;         // the last entry that begins at or before x and is not empty
+        while (r - l > 1) {
+            const uint32_t mid = (l + r) / 2;
+            if (before[mid] <= x) l = mid;
+            else r = mid;
+        }
+        u.e = l;
+        u.t = entry_of(a, u.e, pre_lo, pre_hi);
+        const uint32_t at = x - before[l], seg = at / u.t.steps;
+        u.h = seg / u.t.tiles;
+        u.tile = seg % u.t.tiles;
+        u.step = at % u.t.steps;
+        enter(u);
+    };
+    auto next = [&](Cursor& u, uint32_t x) {   // to step x, the one behind
+        if (++u.step < u.t.steps) return;
+        u.step = 0;
+        if (++u.tile == u.t.tiles) {
+            u.tile = 0;
+            if (++u.h == c.kv_heads) {
+                u.h = 0;
+                if (x >= total) return;
+                do u.e++;
+                while (before[u.e + 1] <= x);
+                u.t = entry_of(a, u.e, pre_lo, pre_hi);
+            }
+        }
+        enter(u);
+    };
+    auto key_of = [&](const Cursor& u) { return (u.t.lo & ~(kBox - 1)) + u.step * kStep; };
+    auto hidden = [&](const Cursor& u) { return key_of(u) >= u.hi || key_of(u) + kStep <= u.lo; };      // from all rows of the tile
+
+    const uint32_t bar0 = smem_u32(&bars[warp * S::kStages]), ring0 = smem_u32(ring) + warp * S::kStages * S::kStage;
+    Cursor in, at;
+    seek(at, x0);
+    in = at;
+    int32_t page[2];
+    auto look_up = [&]() {                     // pages of the copier's next step
+        const uint32_t k = key_of(in);
+#pragma unroll
+        for (uint32_t b = 0; b < 2; b++) page[b] = k + b * kBox < in.hi ? in.t.table[(k + b * kBox) >> c.page_log2] : 0;
+    };
+    auto copy = [&](uint32_t stage) {
+        const uint32_t k = key_of(in), n = hidden(in) ? 0 : k + kBox < in.hi ? 2 : 1;
+#pragma unroll
+        for (uint32_t b = 0; b < 2; b++)
+            if (b < n && (uint32_t)page[b] >= c.n_pages) {
+                report(c);
+                page[b] = 0;
+            }
+        if (lane == 0) {
+            const uint32_t bar = bar0 + 8 * stage, dst = ring0 + stage * S::kStage;
+            mbar_expect_tx(bar, n * 2 * S::kBoxBytes);
+#pragma unroll
+            for (uint32_t b = 0; b < 2; b++) {
+                if (b >= n) break;
+                const uint32_t p = k + b * kBox;
+                const int32_t row = (int32_t)((((uint32_t)page[b] * c.kv_heads + in.h) << c.page_log2) + (p & ((1u << c.page_log2) - 1)));
+                tma_load_3d(dst + b * S::kBoxBytes, &mk, 0, row, 0, bar);
+                tma_load_3d(dst + (2 + b) * S::kBoxBytes, &mv, 0, row, 0, bar);
+            }
+        }
+        __syncwarp();
+    };
+    uint32_t xin = x0;
+    look_up();
+    for (uint32_t s = 0; s < S::kStages && xin < x1; s++) {
+        copy(s);
+        xin++;
+        next(in, xin);
+        if (xin < x1) look_up();
+    }
+
+    uint32_t qa[KS][4], lo[2], hi[2];
+    int32_t pos[2];
+    size_t orow[2];                            // (row, head) of a thread's two rows
+    bool live[2];
+    float o[ND][4], m[2], l[2];
+    Scoring sc;
+    sc.cap = a.cap;
+    sc.inv_cap = a.cap != 0.f ? 1.f / a.cap : 0.f;
+    sc.plain = a.cap == 0.f && !a.slopes;
+    sc.mul = sc.plain ? a.scale * kLog2e : a.scale;
+    auto begin = [&]() {                       // rows of the reader's segment
+#pragma unroll
+        for (uint32_t r = 0; r < 2; r++) {
+            const uint32_t i = at.tile * kRows + g4 + 8 * r;
+            live[r] = i < at.t.n * c.group;
+            const uint32_t token = at.t.row0 + (live[r] ? i / c.group : 0), head = at.h * c.group + (live[r] ? i % c.group : 0);
+            pos[r] = at.t.base + (int32_t)(i / c.group);
+            uint32_t limit = 0x7FFFFFFFu;
+            if (at.e >= c.n_seqs && live[r]) {
+                const uint32_t s = sequence_by_halves(c, token);
+                live[r] = s < c.n_seqs;
+                if (live[r]) {
+                    const Seq q = sequence(c, s);
+                    live[r] = token >= q.row0 && token < q.row0 + q.n;
+                    pos[r] = (int32_t)q.len - (int32_t)(q.row0 + q.n - token);
+                }
+                limit = c.shared;
+            }
+            orow[r] = (size_t)token * c.heads + head;
+            lo[r] = live[r] ? first_seen(pos[r], a.window) : 0;
+            if (live[r] && at.e < c.n_seqs) lo[r] = max(lo[r], c.shared);
+            hi[r] = live[r] ? min((uint32_t)max(0, pos[r] + 1), limit) : 0x7FFFFFFFu;
+            (r ? sc.slope1 : sc.slope0) = a.slopes && live[r] ? a.slopes[head] : 0.f;
+            const uint32_t* qp = reinterpret_cast<const uint32_t*>(reinterpret_cast<const T*>(a.q) + (size_t)token * a.ldq + (size_t)head * HD);
+#pragma unroll
+            for (uint32_t k = 0; k < KS; k++) {
+                qa[k][r] = live[r] ? qp[8 * k + t4] : 0;
+                qa[k][2 + r] = live[r] ? qp[8 * k + 4 + t4] : 0;
+            }
+            m[r] = -INFINITY;
+            l[r] = 0.f;
+        }
+#pragma unroll
+        for (uint32_t d = 0; d < ND; d++) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+    };
+    // `whole`: this worker has had all steps of the segment
+    auto finish = [&](bool whole, bool first) {
+#pragma unroll
+        for (uint32_t r = 0; r < 2; r++) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            if (!live[r]) continue;
+            if (whole && n_entries == c.n_seqs && c.shared == 0) {
+                const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+                uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + orow[r] / c.heads * a.ldo + orow[r] % c.heads * HD);
+#pragma unroll
+                for (uint32_t d = 0; d < ND; d++) dst[4 * d + t4] = Half2<T>::pack(o[d][2 * r] * inv, o[d][2 * r + 1] * inv);
+                continue;
+            }
+            float *po, *pml;
+            if (whole) {
+                const bool pre = at.e >= c.n_seqs;
+                po = (pre ? a.pre_o : a.row_o) + orow[r] * HD;
+                pml = (pre ? a.pre_ml : a.row_ml) + orow[r] * 2;
+            } else {
+                const Piece p = slot_of(a, me, first);
+                po = p.o + (g4 + 8 * r) * HD;
+                pml = p.ml + (g4 + 8 * r) * 2;
+            }
+#pragma unroll
+            for (uint32_t d = 0; d < ND; d++) *reinterpret_cast<float2*>(po + 8 * d + 2 * t4) = make_float2(o[d][2 * r], o[d][2 * r + 1]);
+            if (t4 == 0) *reinterpret_cast<float2*>(pml) = make_float2(m[r], l[r]);
+        }
+    };
+
+    bool ok = true;
+    uint32_t begun = x0 - at.step;             // where the segment begins in the order of steps
+    begin();
+    for (uint32_t x = x0; x < x1 && ok; x++) {
+        const uint32_t n = x - x0, stage = n % S::kStages;
+        ok = __all_sync(0xffffffffu, mbar_wait(bar0 + 8 * stage, (n / S::kStages) & 1));
+        if (!ok) break;
+        const uint32_t k0 = key_of(at);
+        if (!hidden(at)) {
+            const uint32_t sk = ring0 + stage * S::kStage, sv = sk + 2 * S::kBoxBytes;
+            float s[NK][4];
+#pragma unroll
+            for (uint32_t j = 0; j < NK; j++) {
+                s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+                const uint32_t row = (j & 1) * 8 + (lane & 7);
+#pragma unroll
+                for (uint32_t k = 0; k < KS; k += 2) {
+                    uint32_t b[4];
+                    const uint32_t ch = 2 * k + (lane >> 3);                        // 16-byte piece of the key's row
+                    ldsm_x4(b, sk + (j >> 1) * S::kBoxBytes + (ch >> 3) * (kBox * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
+                    Half2<T>::mma(s[j], qa[k], b[0], b[1]);
+                    Half2<T>::mma(s[j], qa[k + 1], b[2], b[3]);
+                }
+            }
+            // a thread has keys 8 j + 2 t4, + 1 of rows g4 and g4 + 8
+            const bool inside = k0 >= lo[0] && k0 >= lo[1] && k0 + kStep <= hi[0] && k0 + kStep <= hi[1];
+            const bool all = __all_sync(0xffffffffu, inside);
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (uint32_t j = 0; j < NK; j++)
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) {
+                    const uint32_t r = e >> 1, key = k0 + 8 * j + 2 * t4 + (e & 1);
+                    float v = score(sc, s[j][e], r ? sc.slope1 : sc.slope0, (float)(pos[r] - (int32_t)key));
+                    if (!all && (key < lo[r] || key >= hi[r])) v = -INFINITY;
+                    s[j][e] = v;
+                    top[r] = fmaxf(top[r], v);
+                }
+            float corr[2];
+            bool rise = false;
+#pragma unroll
+            for (uint32_t r = 0; r < 2; r++) {
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                const float now = fmaxf(m[r], top[r]);
+                corr[r] = now > m[r] ? exp2_approx(m[r] - now) : 1.f;
+                rise |= now > m[r];
+                m[r] = now;
+                l[r] *= corr[r];
+            }
+            if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+                for (uint32_t d = 0; d < ND; d++) {
+                    o[d][0] *= corr[0];
+                    o[d][1] *= corr[0];
+                    o[d][2] *= corr[1];
+                    o[d][3] *= corr[1];
+                }
+            }
+            const float sub[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+#pragma unroll
+            for (uint32_t j = 0; j < NK; j++)
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) {
+                    s[j][e] = exp2_approx(s[j][e] - sub[e >> 1]);
+                    l[e >> 1] += s[j][e];
+                }
+            uint32_t bad = 0;
+#pragma unroll
+            for (uint32_t k = 0; k < kStep / 16; k++) {
+                // the weights meet the values in the cache's type: half a step of it, relative, each; their sum is that of the 32-bit ones
+                const uint32_t pa[4] = {Half2<T>::pack(s[2 * k][0], s[2 * k][1]), Half2<T>::pack(s[2 * k][2], s[2 * k][3]), Half2<T>::pack(s[2 * k + 1][0], s[2 * k + 1][1]),
+                                        Half2<T>::pack(s[2 * k + 1][2], s[2 * k + 1][3])};
+                const uint32_t row = ((lane >> 3) & 1) * 8 + (lane & 7);
+#pragma unroll
+                for (uint32_t d = 0; d < ND; d += 2) {
+                    uint32_t b[4];
+                    const uint32_t ch = d + (lane >> 4);
+                    ldsm_x4_trans(b, sv + k * S::kBoxBytes + (ch >> 3) * (kBox * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
+                    if (!all) {                // a hidden position's weight of 0 would meet whatever lies there, and 0 x Inf is NaN
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; i++) {
+                            const uint32_t nf = Half2<T>::not_finite(b[i]);
+                            b[i] = finite_part<T>(b[i], nf);
+                            bad |= nf;
+                        }
+                    }
+                    Half2<T>::mma(o[d], pa, b[0], b[1]);
+                    Half2<T>::mma(o[d + 1], pa, b[2], b[3]);
+                }
+            }
+            if (!all && __any_sync(0xffffffffu, bad != 0))
+                add_not_finite<T, HD>(ring + warp * S::kStages * S::kStage + stage * S::kStage + 2 * S::kBoxBytes, k0, at.hi, lo, hi, s, o);
+        }
+        __syncwarp();
+        if (xin < x1) {
+            copy(stage);
+            xin++;
+            next(in, xin);
+            if (xin < x1) look_up();
+        }
+        const uint32_t left = at.t.steps - at.step - 1;
+        if (left == 0 || x + 1 == x1) {
+            finish(left == 0 && begun >= x0, begun <= x0);
+            next(at, x + 1);
+            begun = x + 1;
+            if (x + 1 < x1) begin();
+        } else next(at, x + 1);
+    }
+    if (!ok) {
+        mbar_drain(bar0, S::kStages, xin - x0);
+        if (lane == 0 && c.status) atomicCAS(c.status, 0, 1);
+    }
+}
+
+// Adds up the pieces of a (row, query head): a block for each, its warps take the pieces in turn, a lane 2 or 4 of the dimensions.  Rows that a worker has
+// written itself are left.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) merge_kernel(const AttnArgs a, const uint32_t n_entries) {
+    constexpr uint32_t E = HD / 32;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    __shared__ float sm[8], sl[8], so[8][HD];
+    const Cache& c = a.c;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5, head = blockIdx.x % c.heads, token = blockIdx.x / c.heads;
+    const uint32_t s = sequence_by_halves(c, token);
+    if (s >= c.n_seqs) return;
+    const uint32_t pre_lo = a.plan[0], pre_hi = a.plan[1], workers = a.plan[2], total = a.plan[kPlanHead + n_entries];
+    const Entry t = entry_of(a, s, pre_lo, pre_hi);
+    if (token < t.row0 || token >= t.row0 + t.n) return;
+    const uint32_t h = head / c.group, gi = head % c.group;
+    float m = -INFINITY, l = 0.f, o[E];
+#pragma unroll
+    for (uint32_t e = 0; e < E; e++) o[e] = 0.f;
+    auto add = [&](const float* po, const float* pml) {
+        const float2 ml = *reinterpret_cast<const float2*>(pml);
+        float v[E];
+        if constexpr (E == 4) {
+            const float4 x = *reinterpret_cast<const float4*>(po + 4 * lane);
+            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+        } else {
+            const float2 x = *reinterpret_cast<const float2*>(po + 2 * lane);
+            v[0] = x.x; v[1] = x.y;
+        }
+        const float now = fmaxf(m, ml.x);      // no score yet: the sums are 0, or no numbers
+        const float f0 = now == -INFINITY ? 1.f : exp2_approx(m - now), f1 = now == -INFINITY ? 1.f : exp2_approx(ml.x - now);
+        m = now;
+        l = l * f0 + ml.y * f1;
+#pragma unroll
+        for (uint32_t e = 0; e < E; e++) o[e] = o[e] * f0 + v[e] * f1;
+    };
+    // pieces of one entry's segment that holds row i of the entry
+    auto entry_pieces = [&](const Entry& u, uint32_t e, uint32_t i, const float* whole_o, const float* whole_ml) -> bool {
+        if (u.steps == 0) return true;
+        const uint32_t beg = a.plan[kPlanHead + e] + (h * u.tiles + i / kRows) * u.steps, w0 = owner_of(beg, total, workers), w1 = owner_of(beg + u.steps - 1, total, workers);
+        if (w0 == w1) {
+            if (c.shared == 0) return false;
+            if (warp == 0) add(whole_o, whole_ml);
+            return true;
+        }
+        for (uint32_t w = w0 + warp; w <= w1; w += warps) {
+            const Piece p = slot_of(a, w, begin_of(w, total, workers) >= beg);
+            add(p.o + (i % kRows) * HD, p.ml + (i % kRows) * 2);
+        }
+        return true;
+    };
+    const size_t orow = (size_t)token * c.heads + head;
+    if (!entry_pieces(t, s, (token - t.row0) * c.group + gi, a.row_o + orow * HD, a.row_ml + orow * 2)) return;
+    if (n_entries > c.n_seqs) entry_pieces(entry_of(a, c.n_seqs, pre_lo, pre_hi), c.n_seqs, token * c.group + gi, a.pre_o + orow * HD, a.pre_ml + orow * 2);
+    if (warps > 1) {
+        if (lane == 0) { sm[warp] = m; sl[warp] = l; }
+#pragma unroll
+        for (uint32_t e = 0; e < E; e++) so[warp][E * lane + e] = o[e];
+        __syncthreads();
+        if (warp > 0) return;
+        for (uint32_t w = 1; w < warps; w++) {
+            const float2 ml = make_float2(sm[w], sl[w]);
+            const float now = fmaxf(m, ml.x);
+            const float f0 = now == -INFINITY ? 1.f : exp2_approx(m - now), f1 = now == -INFINITY ? 1.f : exp2_approx(ml.x - now);
+            m = now;
+            l = l * f0 + ml.y * f1;
+#pragma unroll
+            for (uint32_t e = 0; e < E; e++) o[e] = o[e] * f0 + so[w][E * lane + e] * f1;
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + (size_t)token * a.ldo + (size_t)head * HD);
+#pragma unroll
+    for (uint32_t e = 0; e < E / 2; e++) dst[lane * (E / 2) + e] = Half2<T>::pack(o[2 * e] * inv, o[2 * e + 1] * inv);
+}
+
+// ── the scratch ──
+struct Layout {
+    size_t plan, slot_o, slot_ml, row_o, row_ml, pre_o, pre_ml, bytes;
+};
+static Layout layout_of(const runit_paged_cfg* g, const runit_paged_batch* b) {
+    Layout l;
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        const size_t p = at;
+        at += (n + 255) & ~(size_t)255;
+        return p;
+    };
+    const size_t pairs = b->shared_len ? (size_t)b->rows * g->heads : 0;
+    l.plan = take((kPlanHead + kMaxSeqs + 2) * 4);
+    l.slot_o = take((size_t)2 * kMaxWorkers * kRows * g->dim * 4);
+    l.slot_ml = take((size_t)2 * kMaxWorkers * kRows * 8);
+    l.row_o = take(pairs * g->dim * 4);
+    l.row_ml = take(pairs * 8);
+    l.pre_o = take(pairs * g->dim * 4);
+    l.pre_ml = take(pairs * 8);
+    l.bytes = at;
+    return l;
+}
+
+static int32_t encode(runit_ctx* ctx, const runit_paged_cfg* g, void* pages, CUtensorMap* m) {
+    if (!ctx->encode_tiled) return runit_fail(ctx, RUNIT_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled is not available");
+    auto f = reinterpret_cast<CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                           const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill)>(ctx->encode_tiled);
+    const cuuint64_t dim[3] = {64, (cuuint64_t)g->n_pages * g->kv_heads * g->page, g->dim / 64}, stride[2] = {g->dim * 2ull, 128};
+    const cuuint32_t box[3] = {64, kBox, g->dim / 64}, one[3] = {1, 1, 1};
+    const CUresult r = f(m, g->type == RUNIT_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, pages, dim, stride, box, one,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return runit_fail(ctx, RUNIT_ERR_LAUNCH, "cuTensorMapEncodeTiled failed with %d", (int)r);
+    return RUNIT_OK;
+}
+
+template <typename T, int HD>
+static int32_t run(runit_ctx* ctx, const runit_paged_cfg* g, const runit_paged_batch* b, const AttnArgs& a) {
+    constexpr uint32_t smem = Shape<HD>::kRing + 1024 + (kMaxSeqs + 2) * 4;
+    static bool configured[64] = {false};
+    if (ctx->device >= 64 || !configured[ctx->device]) {
+        RUNIT_CUDA_TRY(ctx, cudaFuncSetAttribute(paged_split_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        if (ctx->device < 64) configured[ctx->device] = true;
+    }
+    CUtensorMap mk, mv;
+    int32_t st = encode(ctx, g, g->k_pages, &mk);
+    if (st == RUNIT_OK) st = encode(ctx, g, g->v_pages, &mv);
+    if (st != RUNIT_OK) return st;
+    const uint32_t grid = min((uint32_t)ctx->sm_count, kMaxWorkers / kWarps), n_entries = b->n_seqs + (b->shared_len ? 1 : 0);
+    runit_launch_chain_smem(ctx, paged_split_kernel<T, HD>, dim3(grid), dim3(kWarps * 32), smem, mk, mv, a, n_entries);
+    if ((st = runit_after_launch(ctx, "paged_attention")) != RUNIT_OK) return st;
+    // warps of a merging block: about as many as a segment has pieces when all are alike
+    const uint32_t share = grid * kWarps / max(1u, b->n_seqs * g->kv_heads), warps = share >= 8 ? 8 : share >= 2 ? 4 : 1;
+    runit_launch_chain(ctx, merge_kernel<T, HD>, dim3(g->heads * b->rows), dim3(32 * warps), a, n_entries);
+    return runit_after_launch(ctx, "paged_attention (merge)");
 }
 
 }  // namespace pg
@@ -75,7 +603,9 @@ using namespace runit;
 
 extern "C" {
 
-size_t runit_paged_attention_scratch_bytes(const runit_paged_cfg* cfg, const runit_paged_batch* batch) { return pg::why_not(cfg, batch) ? 0 : 1024; }
+size_t runit_paged_attention_scratch_bytes(const runit_paged_cfg* cfg, const runit_paged_batch* batch) {
+    return pg::why_not(cfg, batch) ? 0 : pg::layout_of(cfg, batch).bytes;
+}
 
 int32_t runit_paged_attention(runit_ctx_t* ctx, const runit_paged_cfg* cfg, const runit_paged_batch* batch, const void* q, uint32_t ldq, void* out,
                               uint32_t ldo, void* scratch, size_t scratch_bytes) {
@@ -87,18 +617,13 @@ int32_t runit_paged_attention(runit_ctx_t* ctx, const runit_paged_cfg* cfg, cons
     RUNIT_REQUIRE(ctx, ldq % 8 == 0 && ldo % 8 == 0 && ldq >= (uint64_t)cfg->heads * cfg->dim && ldo >= (uint64_t)cfg->heads * cfg->dim,
                   "paged_attention: ldq=%u, ldo=%u must be multiples of 8, rows of heads * dim at least", ldq, ldo);
     RUNIT_REQUIRE(ctx, scratch && runit_aligned(scratch, 256), "paged_attention: scratch must be 256-byte aligned");
-    if (scratch_bytes < runit_paged_attention_scratch_bytes(cfg, batch))
-        return runit_fail(ctx, RUNIT_ERR_BUFFER_SIZE, "paged_attention: %zu bytes of scratch, %zu needed", scratch_bytes, runit_paged_attention_scratch_bytes(cfg, batch));
-    const pg::AttnArgs a{pg::cache_of(ctx, cfg, batch), q, out, (const float*)cfg->slopes, ldq, ldo, cfg->window, cfg->scale, cfg->cap};
-    const dim3 grid(batch->rows, cfg->heads);
-    if (cfg->type == RUNIT_TYPE_F16) {
-        if (cfg->dim == 128) runit_launch_chain(ctx, pg::paged_attention_kernel<__half, 128>, grid, dim3(128), a);
-        else runit_launch_chain(ctx, pg::paged_attention_kernel<__half, 64>, grid, dim3(128), a);
-    } else {
-        if (cfg->dim == 128) runit_launch_chain(ctx, pg::paged_attention_kernel<__nv_bfloat16, 128>, grid, dim3(128), a);
-        else runit_launch_chain(ctx, pg::paged_attention_kernel<__nv_bfloat16, 64>, grid, dim3(128), a);
-    }
-    return runit_after_launch(ctx, "paged_attention");
+    const pg::Layout l = pg::layout_of(cfg, batch);
+    if (scratch_bytes < l.bytes) return runit_fail(ctx, RUNIT_ERR_BUFFER_SIZE, "paged_attention: %zu bytes of scratch, %zu needed", scratch_bytes, l.bytes);
+    uint8_t* const s = (uint8_t*)scratch;
+    const pg::AttnArgs a{pg::cache_of(ctx, cfg, batch), q, out, (const float*)cfg->slopes, ldq, ldo, cfg->window, cfg->scale, cfg->cap, (uint32_t*)(s + l.plan),
+                         (float*)(s + l.slot_o), (float*)(s + l.slot_ml), (float*)(s + l.row_o), (float*)(s + l.row_ml), (float*)(s + l.pre_o), (float*)(s + l.pre_ml)};
+    if (cfg->type == RUNIT_TYPE_F16) return cfg->dim == 128 ? pg::run<__half, 128>(ctx, cfg, batch, a) : pg::run<__half, 64>(ctx, cfg, batch, a);
+    return cfg->dim == 128 ? pg::run<__nv_bfloat16, 128>(ctx, cfg, batch, a) : pg::run<__nv_bfloat16, 64>(ctx, cfg, batch, a);
 }
 
 }  // extern "C"

@@ -1,0 +1,90 @@
+// What the kernels of the attention over a paged cache share: arguments, places in the scratch, the products of the legacy tensor path, and the
+// operations on scores.
+#pragma once
+
+#include "gemv_common.cuh"
+#include "paged.cuh"
+#include "tma.cuh"
+
+namespace runit {
+namespace pg {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttnArgs {
+    Cache c;
+    const void* q;
+    void* out;
+    const float* slopes;
+    uint32_t ldq, ldo, window;
+    float scale, cap;
+    // scratch
+    uint32_t* plan;          // kPlanHead words, then the steps in front of every entry
+    float *slot_o, *slot_ml; // [2 * workers][16][dim] and [..][16][2]: pieces of segments that workers share
+    float *row_o, *row_ml;   // [rows * heads][dim] and [..][2]: what one worker has of a row whose shared positions come from elsewhere
+    float *pre_o, *pre_ml;   // the same for the shared positions (as many times as they are split)
+};
+
+__device__ __forceinline__ float exp2_approx(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int32_t c0, int32_t c1, int32_t c2, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+}
+// What differs between the two 16-bit types: products, packing, and bits that are no number.
+template <typename T> struct Half2;
+template <> struct Half2<__half> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+    static __device__ __forceinline__ uint32_t not_finite(uint32_t w) { return ((w & 0x7FFF7FFFu) + 0x04000400u) & 0x80008000u; }
+    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+template <> struct Half2<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+    static __device__ __forceinline__ uint32_t not_finite(uint32_t w) { return ((w & 0x7FFF7FFFu) + 0x00800080u) & 0x80008000u; }
+    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+// the 16-bit halves of w that are no numbers, set to zero
+template <typename T> __device__ __forceinline__ uint32_t finite_part(uint32_t w, uint32_t nf) { return w & ~((nf >> 15) * 0xFFFFu); }
+
+// The first position that the one at `pos` sees.
+__device__ __forceinline__ uint32_t first_seen(int32_t pos, uint32_t window) { return window && pos >= 0 && (uint32_t)pos >= window ? (uint32_t)pos + 1 - window : 0; }
+// Sequence of a row by halving the starts; c.n_seqs: nobody's.
+__device__ __forceinline__ uint32_t sequence_by_halves(const Cache& c, uint32_t row) {
+    uint32_t lo = 0, hi = c.n_seqs;            // as many of q_start[1 ..] as are <= row
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (c.q_start[mid + 1] <= (int32_t)row) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+}  // namespace pg
+}  // namespace runit

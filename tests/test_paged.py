@@ -19,7 +19,7 @@ def _described(**change):
 @pytest.mark.parametrize("change", [dict(heads=0), dict(heads=30), dict(heads=1028), dict(kv_heads=0), dict(dim=32), dict(dim=256), dict(page=0), dict(page=48), dict(page=8),
                                     dict(page=512), dict(n_pages=0), dict(n_pages=0xFFFFFFFF), dict(n_pages=1 << 24), dict(type=0), dict(type=3), dict(scale=float("inf")),
                                     dict(cap=float("nan")), dict(cap=-2.0), dict(n_seqs=0), dict(n_seqs=5000), dict(rows=0), dict(rows=1 << 28), dict(table_ld=0),
-                                    dict(table_ld=1 << 26), dict(shared_len=63), dict(shared_len=6464)])
+                                    dict(table_ld=1 << 26), dict(shared_len=63), dict(shared_len=6464), dict(n_seqs=4096, table_ld=1 << 20)])
 def test_descriptions_that_are_refused(change):
     assert _described(**change) == 0
 
