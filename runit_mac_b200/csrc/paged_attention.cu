@@ -1,7 +1,7 @@
 // Attention of a batch of sequences over a paged cache: out_i = sum_j softmax_j(s_ij) v_j over the positions j that row i sees, s_ij = scale q_i . k_j,
 // then cap * tanh(s / cap), then minus slope * (i - j).
 //
-// Few rows a sequence (decoding): bound by HBM, which has to deliver every key and value once.  A segment is what shares keys: up to 16 (row, query head)
+// Many rows that share keys: paged_attention_tc.cu.  Few rows a sequence (decoding): bound by HBM, which has to deliver every key and value once.  A segment is what shares keys: up to 16 (row, query head)
 // pairs of one sequence and key head, and the positions that they see; the segments' steps of 32 positions, one behind the other, are dealt out evenly to
 // the warps of the grid, whatever the lengths.  A warp is on its own: it copies its steps by TMA into a ring (boxes of 16 positions, so that pages of
 // 16 are whole boxes), multiplies on the legacy tensor path with the rows as m16 (a tcgen05 tile would be 128 rows, mostly padding), and keeps
@@ -65,19 +65,6 @@ __device__ __forceinline__ Piece slot_of(const AttnArgs& a, uint32_t w, bool fir
     return Piece{a.slot_o + s * kRows * a.c.dim, a.slot_ml + s * kRows * 2};
 }
 
-// ── operations on scores ──
-struct Scoring {
-    float mul, cap, inv_cap, slope0, slope1;   // mul: scale (times log2 e without cap and bias); slopes of a thread's two rows
-    bool plain;
-};
-// A score in units of log2: x[row][key].
-__device__ __forceinline__ float score(const Scoring& s, float dot, float slope, float back) {
-    if (s.plain) return dot * s.mul;
-    float t = dot * s.mul;
-    if (s.cap != 0.f) t = s.cap * tanhf(t * s.inv_cap);
-    return (t - slope * back) * kLog2e;
-}
-
 // V of a step whose hidden positions hold something that is no number: its elements were left out of the products (0 there), the rows that see
 // them get them here.  p: the weights as the products' accumulators hold them.
 template <typename T, int HD>
@@ -116,7 +103,7 @@ __device__ __noinline__ void add_not_finite(const uint8_t* stage_v, uint32_t k0,
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const AttnArgs a,
-                                                                   const uint32_t n_entries) {
+                                                                   const uint32_t e0, const uint32_t n_entries) {
     using S = Shape<HD>;
     constexpr uint32_t KS = HD / 16, ND = HD / 8, NK = kStep / 8;
     extern __shared__ uint8_t smem_raw[];
@@ -136,7 +123,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
     grid_dependency_wait();
     grid_launch_dependents();
     // the shared positions that some row sees
-    if (n_entries > c.n_seqs) {
+    if (e0 + n_entries > c.n_seqs) {
         uint32_t lo = c.shared, hi = 0;
         for (uint32_t e = tid; e < c.n_seqs; e += kWarps * 32) {
             const Seq s = sequence(c, e);
@@ -153,7 +140,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
         const uint32_t per = (n_entries + kWarps * 32 - 1) / (kWarps * 32), beg = min(n_entries, tid * per), end = min(n_entries, beg + per);
         uint32_t sum = 0;
         for (uint32_t e = beg; e < end; e++) {
-            const Entry t = entry_of(a, e, pre_lo, pre_hi);
+            const Entry t = entry_of(a, e0 + e, pre_lo, pre_hi);
             before[e] = sum;
             sum += t.tiles * t.steps * c.kv_heads;
         }
@@ -178,6 +165,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
             a.plan[0] = pre_lo;
             a.plan[1] = pre_hi;
             a.plan[2] = workers;
+            a.plan[3] = e0;
+            a.plan[4] = total;
         }
     }
     const uint32_t me = warp * gridDim.x + blockIdx.x;          // neighbours in the order of steps sit on other SMs: few steps spread over all of them
@@ -206,7 +195,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
             if (before[mid] <= x) l = mid;
             else r = mid;
         }
-        u.e = l;
+        u.e = e0 + l;
         u.t = entry_of(a, u.e, pre_lo, pre_hi);
         const uint32_t at = x - before[l], seg = at / u.t.steps;
         u.h = seg / u.t.tiles;
@@ -223,7 +212,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
                 u.h = 0;
                 if (x >= total) return;
                 do u.e++;
-                while (before[u.e + 1] <= x);
+                while (before[u.e - e0 + 1] <= x);
                 u.t = entry_of(a, u.e, pre_lo, pre_hi);
             }
         }
@@ -278,11 +267,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
     size_t orow[2];                            // (row, head) of a thread's two rows
     bool live[2];
     float o[ND][4], m[2], l[2];
-    Scoring sc;
-    sc.cap = a.cap;
-    sc.inv_cap = a.cap != 0.f ? 1.f / a.cap : 0.f;
-    sc.plain = a.cap == 0.f && !a.slopes;
-    sc.mul = sc.plain ? a.scale * kLog2e : a.scale;
+    // scores times mul are in units of log2; plain: products are scores times a positive scale.  Else they are scaled (before the cap or here) and biased.
+    const bool plain = a.cap == 0.f && !a.slopes && a.scale > 0.f;
+    const float mul = plain ? a.scale * kLog2e : kLog2e, pre = a.cap != 0.f ? 1.f : a.scale, inv_cap = a.cap != 0.f ? 1.f / a.cap : 0.f;
+    float slope[2];
     auto begin = [&]() {                       // rows of the reader's segment
 #pragma unroll
         for (uint32_t r = 0; r < 2; r++) {
@@ -305,7 +293,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
             lo[r] = live[r] ? first_seen(pos[r], a.window) : 0;
             if (live[r] && at.e < c.n_seqs) lo[r] = max(lo[r], c.shared);
             hi[r] = live[r] ? min((uint32_t)max(0, pos[r] + 1), limit) : 0x7FFFFFFFu;
-            (r ? sc.slope1 : sc.slope0) = a.slopes && live[r] ? a.slopes[head] : 0.f;
+            slope[r] = a.slopes && live[r] ? a.slopes[head] : 0.f;
             const uint32_t* qp = reinterpret_cast<const uint32_t*>(reinterpret_cast<const T*>(a.q) + (size_t)token * a.ldq + (size_t)head * HD);
 #pragma unroll
             for (uint32_t k = 0; k < KS; k++) {
@@ -325,7 +313,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
             if (!live[r]) continue;
-            if (whole && n_entries == c.n_seqs && c.shared == 0) {
+            if (whole && c.shared == 0) {
                 const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
                 uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + orow[r] / c.heads * a.ldo + orow[r] % c.heads * HD);
 #pragma unroll
@@ -376,22 +364,30 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
             const bool inside = k0 >= lo[0] && k0 >= lo[1] && k0 + kStep <= hi[0] && k0 + kStep <= hi[1];
             const bool all = __all_sync(0xffffffffu, inside);
             float top[2] = {-INFINITY, -INFINITY};
+            if (!plain || !all) {
+                if (a.cap != 0.f) cap_scores(reinterpret_cast<float(&)[4 * NK]>(s), a.scale, a.cap, inv_cap);
+                // in units of mul afterwards, like the plain ones
+#pragma unroll
+                for (uint32_t j = 0; j < NK; j++)
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; e++) {
+                        const uint32_t r = e >> 1, key = k0 + 8 * j + 2 * t4 + (e & 1);
+                        float v = plain ? s[j][e] : s[j][e] * pre - slope[r] * (float)(pos[r] - (int32_t)key);
+                        if (key < lo[r] || key >= hi[r]) v = -INFINITY;
+                        s[j][e] = v;
+                    }
+            }
 #pragma unroll
             for (uint32_t j = 0; j < NK; j++)
 #pragma unroll
-                for (uint32_t e = 0; e < 4; e++) {
-                    const uint32_t r = e >> 1, key = k0 + 8 * j + 2 * t4 + (e & 1);
-                    float v = score(sc, s[j][e], r ? sc.slope1 : sc.slope0, (float)(pos[r] - (int32_t)key));
-                    if (!all && (key < lo[r] || key >= hi[r])) v = -INFINITY;
-                    s[j][e] = v;
-                    top[r] = fmaxf(top[r], v);
-                }
+                for (uint32_t e = 0; e < 4; e++) top[e >> 1] = fmaxf(top[e >> 1], s[j][e]);
             float corr[2];
             bool rise = false;
 #pragma unroll
             for (uint32_t r = 0; r < 2; r++) {
                 top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
                 top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                top[r] *= mul;
                 const float now = fmaxf(m[r], top[r]);
                 corr[r] = now > m[r] ? exp2_approx(m[r] - now) : 1.f;
                 rise |= now > m[r];
@@ -408,16 +404,24 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
                 }
             }
             const float sub[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+            // the product's rounding against that of the maximum (2^-24 of the score) stays in the weight, as an f32 score's own would
 #pragma unroll
             for (uint32_t j = 0; j < NK; j++)
 #pragma unroll
                 for (uint32_t e = 0; e < 4; e++) {
-                    s[j][e] = exp2_approx(s[j][e] - sub[e >> 1]);
+                    s[j][e] = exp2_approx(fmaf(s[j][e], mul, -sub[e >> 1]));
                     l[e >> 1] += s[j][e];
                 }
             uint32_t bad = 0;
 #pragma unroll
             for (uint32_t k = 0; k < kStep / 16; k++) {
+                if (k0 + 16 * k >= at.hi) break;                // not copied
+                // of the two keys in a word of V: the bits of those that some row of the tile sees
+                const uint32_t ka = k0 + 16 * k + 2 * t4;
+                uint32_t seen[2];
+#pragma unroll
+                for (uint32_t i = 0; i < 2; i++)
+                    seen[i] = (ka + 8 * i >= at.lo && ka + 8 * i < at.hi ? 0x8000u : 0) | (ka + 8 * i + 1 >= at.lo && ka + 8 * i + 1 < at.hi ? 0x80000000u : 0);
                 // the weights meet the values in the cache's type: half a step of it, relative, each; their sum is that of the 32-bit ones
                 const uint32_t pa[4] = {Half2<T>::pack(s[2 * k][0], s[2 * k][1]), Half2<T>::pack(s[2 * k][2], s[2 * k][3]), Half2<T>::pack(s[2 * k + 1][0], s[2 * k + 1][1]),
                                         Half2<T>::pack(s[2 * k + 1][2], s[2 * k + 1][3])};
@@ -432,15 +436,25 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
                         for (uint32_t i = 0; i < 4; i++) {
                             const uint32_t nf = Half2<T>::not_finite(b[i]);
                             b[i] = finite_part<T>(b[i], nf);
-                            bad |= nf;
+                            bad |= nf & seen[i & 1];
                         }
                     }
                     Half2<T>::mma(o[d], pa, b[0], b[1]);
                     Half2<T>::mma(o[d + 1], pa, b[2], b[3]);
                 }
             }
-            if (!all && __any_sync(0xffffffffu, bad != 0))
-                add_not_finite<T, HD>(ring + warp * S::kStages * S::kStage + stage * S::kStage + 2 * S::kBoxBytes, k0, at.hi, lo, hi, s, o);
+            if (!all && __any_sync(0xffffffffu, bad != 0)) {
+                float x[ND][4];                // a copy: what a call is given by address lives in memory from beginning to end
+#pragma unroll
+                for (uint32_t d = 0; d < ND; d++) x[d][0] = o[d][0], x[d][1] = o[d][1], x[d][2] = o[d][2], x[d][3] = o[d][3];
+                float y[NK][4];
+#pragma unroll
+                for (uint32_t j = 0; j < NK; j++) y[j][0] = s[j][0], y[j][1] = s[j][1], y[j][2] = s[j][2], y[j][3] = s[j][3];
+                const uint32_t from[2] = {lo[0], lo[1]}, to[2] = {hi[0], hi[1]};
+                add_not_finite<T, HD>(ring + warp * S::kStages * S::kStage + stage * S::kStage + 2 * S::kBoxBytes, k0, at.hi, from, to, y, x);
+#pragma unroll
+                for (uint32_t d = 0; d < ND; d++) o[d][0] = x[d][0], o[d][1] = x[d][1], o[d][2] = x[d][2], o[d][3] = x[d][3];
+            }
         }
         __syncwarp();
         if (xin < x1) {
@@ -463,75 +477,124 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
     }
 }
 
-// Adds up the pieces of a (row, query head): a block for each, its warps take the pieces in turn, a lane 2 or 4 of the dimensions.  Rows that a worker has
-// written itself are left.
+// Adds up what the launches have left of a (row, query head): a block for each.  First the factors 2^(m - max m) of all pieces, then the sums, the pieces
+// in turn over the block's warps, a lane 2 or 4 of the dimensions.  Rows that a worker has written itself are left.
+struct MergeArgs {
+    uint32_t n_entries;                        // of the split kernel: 0 when it has not run
+    uint32_t own_parts, pre_parts;             // parts of the kernel for many rows: 0 when the split kernel has had those positions
+    const float *own_o, *own_ml, *pre_o, *pre_ml;
+    bool shared;
+};
+constexpr uint32_t kMaxPieces = kMaxWorkers + 640;
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) merge_kernel(const AttnArgs a, const uint32_t n_entries) {
+__global__ void __launch_bounds__(512) merge_kernel(const AttnArgs a, const MergeArgs g) {
     constexpr uint32_t E = HD / 32;
     grid_dependency_wait();
     grid_launch_dependents();
-    __shared__ float sm[8], sl[8], so[8][HD];
+    __shared__ float factor[kMaxPieces], red[2][16], so[16][HD];
     const Cache& c = a.c;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5, head = blockIdx.x % c.heads, token = blockIdx.x / c.heads;
     const uint32_t s = sequence_by_halves(c, token);
     if (s >= c.n_seqs) return;
-    const uint32_t pre_lo = a.plan[0], pre_hi = a.plan[1], workers = a.plan[2], total = a.plan[kPlanHead + n_entries];
-    const Entry t = entry_of(a, s, pre_lo, pre_hi);
-    if (token < t.row0 || token >= t.row0 + t.n) return;
-    const uint32_t h = head / c.group, gi = head % c.group;
+    const size_t orow = (size_t)token * c.heads + head, pairs = (size_t)c.rows * c.heads;
+    // pieces of one entry: as many, from worker w0 on, or one that is whole
+    struct List {
+        uint32_t n, w0, beg, row;
+        bool whole;
+    };
+    uint32_t workers = 1, total = 0;
+    auto list_of = [&](const Entry& u, uint32_t e, uint32_t i) {
+        List x{0, 0, 0, i % kRows, false};
+        if (u.steps == 0) return x;
+        x.beg = a.plan[kPlanHead + e] + (head / c.group * u.tiles + i / kRows) * u.steps;
+        x.w0 = owner_of(x.beg, total, workers);
+        x.n = owner_of(x.beg + u.steps - 1, total, workers) - x.w0 + 1;
+        x.whole = x.n == 1;
+        return x;
+    };
+    List own{g.own_parts, 0, 0, 0, false}, pre{g.pre_parts, 0, 0, 0, false};
+    const Seq q = sequence(c, s);
+    if (token < q.row0 || token >= q.row0 + q.n) return;
+    if (g.n_entries) {
+        const uint32_t pre_lo = a.plan[0], pre_hi = a.plan[1], e0 = a.plan[3];
+        workers = a.plan[2];
+        total = a.plan[4];
+        if (!g.own_parts) {
+            own = list_of(entry_of(a, s, pre_lo, pre_hi), s - e0, (token - q.row0) * c.group + head % c.group);
+            if (own.whole && !g.shared) return;
+        }
+        if (g.shared && !g.pre_parts) pre = list_of(entry_of(a, c.n_seqs, pre_lo, pre_hi), c.n_seqs - e0, token * c.group + head % c.group);
+    }
+    const uint32_t n = own.n + pre.n;
+    auto piece = [&](uint32_t i, const float** po) -> const float* {
+        const bool p = i >= own.n;
+        const List& x = p ? pre : own;
+        if (p) i -= own.n;
+        if (p ? g.pre_parts : g.own_parts) {
+            *po = (p ? g.pre_o : g.own_o) + (i * pairs + orow) * HD;
+            return (p ? g.pre_ml : g.own_ml) + (i * pairs + orow) * 2;
+        }
+        if (x.whole) {
+            *po = (p ? a.pre_o : a.row_o) + orow * HD;
+            return (p ? a.pre_ml : a.row_ml) + orow * 2;
+        }
+        const Piece s = slot_of(a, x.w0 + i, begin_of(x.w0 + i, total, workers) >= x.beg);
+        *po = s.o + x.row * HD;
+        return s.ml + x.row * 2;
+    };
+    auto over_block = [&](float v, bool most, float* r) {
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+            const float t = __shfl_xor_sync(0xffffffffu, v, d);
+            v = most ? fmaxf(v, t) : v + t;
+        }
+        if (warps == 1) return v;
+        if (lane == 0) r[warp] = v;
+        __syncthreads();
+        v = r[0];
+        for (uint32_t w = 1; w < warps; w++) v = most ? fmaxf(v, r[w]) : v + r[w];
+        return v;
+    };
     float m = -INFINITY, l = 0.f, o[E];
+    for (uint32_t i = tid; i < n; i += blockDim.x) {
+        const float* po;
+        const float x = piece(i, &po)[0];
+        factor[i] = x;
+        m = fmaxf(m, x);
+    }
+    m = over_block(m, true, red[0]);
+    for (uint32_t i = tid; i < n; i += blockDim.x) {
+        const float* po;
+        const float f = m == -INFINITY ? 1.f : exp2_approx(factor[i] - m);         // no score at all: the sums are 0, or no numbers
+        factor[i] = f;
+        l = fmaf(f, piece(i, &po)[1], l);
+    }
+    l = over_block(l, false, red[1]);
+    __syncwarp();
 #pragma unroll
     for (uint32_t e = 0; e < E; e++) o[e] = 0.f;
-    auto add = [&](const float* po, const float* pml) {
-        const float2 ml = *reinterpret_cast<const float2*>(pml);
-        float v[E];
+#pragma unroll 4
+    for (uint32_t i = warp; i < n; i += warps) {
+        const float* po;
+        piece(i, &po);
+        const float f = factor[i];
         if constexpr (E == 4) {
             const float4 x = *reinterpret_cast<const float4*>(po + 4 * lane);
-            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+            o[0] = fmaf(f, x.x, o[0]); o[1] = fmaf(f, x.y, o[1]); o[2] = fmaf(f, x.z, o[2]); o[3] = fmaf(f, x.w, o[3]);
         } else {
             const float2 x = *reinterpret_cast<const float2*>(po + 2 * lane);
-            v[0] = x.x; v[1] = x.y;
+            o[0] = fmaf(f, x.x, o[0]); o[1] = fmaf(f, x.y, o[1]);
         }
-        const float now = fmaxf(m, ml.x);      // no score yet: the sums are 0, or no numbers
-        const float f0 = now == -INFINITY ? 1.f : exp2_approx(m - now), f1 = now == -INFINITY ? 1.f : exp2_approx(ml.x - now);
-        m = now;
-        l = l * f0 + ml.y * f1;
-#pragma unroll
-        for (uint32_t e = 0; e < E; e++) o[e] = o[e] * f0 + v[e] * f1;
-    };
-    // pieces of one entry's segment that holds row i of the entry
-    auto entry_pieces = [&](const Entry& u, uint32_t e, uint32_t i, const float* whole_o, const float* whole_ml) -> bool {
-        if (u.steps == 0) return true;
-        const uint32_t beg = a.plan[kPlanHead + e] + (h * u.tiles + i / kRows) * u.steps, w0 = owner_of(beg, total, workers), w1 = owner_of(beg + u.steps - 1, total, workers);
-        if (w0 == w1) {
-            if (c.shared == 0) return false;
-            if (warp == 0) add(whole_o, whole_ml);
-            return true;
-        }
-        for (uint32_t w = w0 + warp; w <= w1; w += warps) {
-            const Piece p = slot_of(a, w, begin_of(w, total, workers) >= beg);
-            add(p.o + (i % kRows) * HD, p.ml + (i % kRows) * 2);
-        }
-        return true;
-    };
-    const size_t orow = (size_t)token * c.heads + head;
-    if (!entry_pieces(t, s, (token - t.row0) * c.group + gi, a.row_o + orow * HD, a.row_ml + orow * 2)) return;
-    if (n_entries > c.n_seqs) entry_pieces(entry_of(a, c.n_seqs, pre_lo, pre_hi), c.n_seqs, token * c.group + gi, a.pre_o + orow * HD, a.pre_ml + orow * 2);
+    }
     if (warps > 1) {
-        if (lane == 0) { sm[warp] = m; sl[warp] = l; }
 #pragma unroll
         for (uint32_t e = 0; e < E; e++) so[warp][E * lane + e] = o[e];
         __syncthreads();
         if (warp > 0) return;
-        for (uint32_t w = 1; w < warps; w++) {
-            const float2 ml = make_float2(sm[w], sl[w]);
-            const float now = fmaxf(m, ml.x);
-            const float f0 = now == -INFINITY ? 1.f : exp2_approx(m - now), f1 = now == -INFINITY ? 1.f : exp2_approx(ml.x - now);
-            m = now;
-            l = l * f0 + ml.y * f1;
+        for (uint32_t w = 1; w < warps; w++)
 #pragma unroll
-            for (uint32_t e = 0; e < E; e++) o[e] = o[e] * f0 + so[w][E * lane + e] * f1;
-        }
+            for (uint32_t e = 0; e < E; e++) o[e] += so[w][E * lane + e];
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + (size_t)token * a.ldo + (size_t)head * HD);
@@ -539,11 +602,46 @@ __global__ void __launch_bounds__(256) merge_kernel(const AttnArgs a, const uint
     for (uint32_t e = 0; e < E / 2; e++) dst[lane * (E / 2) + e] = Half2<T>::pack(o[2 * e] * inv, o[2 * e + 1] * inv);
 }
 
-// ── the scratch ──
-struct Layout {
-    size_t plan, slot_o, slot_ml, row_o, row_ml, pre_o, pre_ml, bytes;
+// ── which kernel has which positions, and the scratch ──
+// By the (row, query head) pairs that share keys: up to 16 (a tile of the split kernel) it is bound by the copies, beyond that it reads its keys again for every
+// 16.  The parts of the kernel for many rows: as many as fill 148 SMs best, of four blocks at least.
+struct Choice {
+    bool own_tc, pre_tc, direct;
+    uint32_t own_tiles, pre_tiles, own_split, pre_split, e0, n_entries;
 };
-static Layout layout_of(const runit_paged_cfg* g, const runit_paged_batch* b) {
+static uint32_t parts_of(uint64_t ctas, uint64_t blocks) {
+    uint32_t best = 1;
+    double most = 0.0;
+    for (uint32_t z = 1; z <= 64 && (z == 1 || z * 4ull <= blocks); z++) {
+        const uint64_t n = ctas * z, waves = (n + 147) / 148;
+        if (z > 1 && n > 2 * 148) break;
+        const double fill = (double)n / (148.0 * (double)waves) - 0.01 * z;         // a part costs its prologue and its sums
+        if (fill > most) {
+            most = fill;
+            best = z;
+        }
+    }
+    return best;
+}
+static Choice choose(const runit_paged_cfg* g, const runit_paged_batch* b) {
+    const uint64_t group = g->heads / g->kv_heads, pairs = b->rows * group;
+    Choice c;
+    c.own_tc = pairs > 32ull * b->n_seqs;
+    c.pre_tc = b->shared_len && pairs > 16;
+    c.own_tiles = (uint32_t)(pairs / 256 + b->n_seqs);
+    c.pre_tiles = (uint32_t)((pairs + 255) / 256);
+    c.own_split = parts_of((pairs / 256 + (b->n_seqs + 1) / 2) * g->kv_heads, (uint64_t)b->table_ld * g->page / 128);
+    c.pre_split = parts_of((uint64_t)c.pre_tiles * g->kv_heads, b->shared_len / 128);
+    c.direct = c.own_tc && !b->shared_len && c.own_split == 1;
+    const bool pre_split_kernel = b->shared_len && !c.pre_tc;
+    c.e0 = c.own_tc ? b->n_seqs : 0;
+    c.n_entries = (c.own_tc ? 0 : b->n_seqs) + (pre_split_kernel ? 1 : 0);
+    return c;
+}
+struct Layout {
+    size_t plan, slot_o, slot_ml, row_o, row_ml, pre_o, pre_ml, own_part_o, own_part_ml, pre_part_o, pre_part_ml, bytes;
+};
+static Layout layout_of(const runit_paged_cfg* g, const runit_paged_batch* b, const Choice& c) {
     Layout l;
     size_t at = 0;
     auto take = [&](size_t n) {
@@ -551,14 +649,19 @@ static Layout layout_of(const runit_paged_cfg* g, const runit_paged_batch* b) {
         at += (n + 255) & ~(size_t)255;
         return p;
     };
-    const size_t pairs = b->shared_len ? (size_t)b->rows * g->heads : 0;
+    const size_t pairs = (size_t)b->rows * g->heads, row = b->shared_len && !c.own_tc ? pairs : 0, pre = b->shared_len && !c.pre_tc ? pairs : 0;
+    const size_t slots = c.n_entries ? 2 * (size_t)kMaxWorkers * kRows : 0, own_parts = c.own_tc && !c.direct ? c.own_split * pairs : 0, pre_parts = c.pre_tc ? c.pre_split * pairs : 0;
     l.plan = take((kPlanHead + kMaxSeqs + 2) * 4);
-    l.slot_o = take((size_t)2 * kMaxWorkers * kRows * g->dim * 4);
-    l.slot_ml = take((size_t)2 * kMaxWorkers * kRows * 8);
-    l.row_o = take(pairs * g->dim * 4);
-    l.row_ml = take(pairs * 8);
-    l.pre_o = take(pairs * g->dim * 4);
-    l.pre_ml = take(pairs * 8);
+    l.slot_o = take(slots * g->dim * 4);
+    l.slot_ml = take(slots * 8);
+    l.row_o = take(row * g->dim * 4);
+    l.row_ml = take(row * 8);
+    l.pre_o = take(pre * g->dim * 4);
+    l.pre_ml = take(pre * 8);
+    l.own_part_o = take(own_parts * g->dim * 4);
+    l.own_part_ml = take(own_parts * 8);
+    l.pre_part_o = take(pre_parts * g->dim * 4);
+    l.pre_part_ml = take(pre_parts * 8);
     l.bytes = at;
     return l;
 }
@@ -576,23 +679,32 @@ static int32_t encode(runit_ctx* ctx, const runit_paged_cfg* g, void* pages, CUt
 }
 
 template <typename T, int HD>
-static int32_t run(runit_ctx* ctx, const runit_paged_cfg* g, const runit_paged_batch* b, const AttnArgs& a) {
-    constexpr uint32_t smem = Shape<HD>::kRing + 1024 + (kMaxSeqs + 2) * 4;
-    static bool configured[64] = {false};
-    if (ctx->device >= 64 || !configured[ctx->device]) {
-        RUNIT_CUDA_TRY(ctx, cudaFuncSetAttribute(paged_split_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        if (ctx->device < 64) configured[ctx->device] = true;
+static int32_t run(runit_ctx* ctx, const runit_paged_cfg* g, const runit_paged_batch* b, const AttnArgs& a, const Choice& c, uint8_t* s, const Layout& l) {
+    int32_t st;
+    const TcArgs pre{min(g->page, 128u), c.pre_split, true, false, (float*)(s + l.pre_part_o), (float*)(s + l.pre_part_ml)};
+    const TcArgs own{min(g->page, 128u), c.own_split, false, c.direct, (float*)(s + l.own_part_o), (float*)(s + l.own_part_ml)};
+    if (c.pre_tc && (st = paged_attention_tc(ctx, g, a, pre, c.pre_tiles)) != RUNIT_OK) return st;
+    if (c.own_tc && (st = paged_attention_tc(ctx, g, a, own, c.own_tiles)) != RUNIT_OK) return st;
+    uint32_t share = 0;
+    if (c.n_entries) {
+        constexpr uint32_t smem = Shape<HD>::kRing + 1024 + (kMaxSeqs + 2) * 4;
+        static bool configured[64] = {false};
+        if (ctx->device >= 64 || !configured[ctx->device]) {
+            RUNIT_CUDA_TRY(ctx, cudaFuncSetAttribute(paged_split_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            if (ctx->device < 64) configured[ctx->device] = true;
+        }
+        CUtensorMap mk, mv;
+        if ((st = encode(ctx, g, g->k_pages, &mk)) != RUNIT_OK || (st = encode(ctx, g, g->v_pages, &mv)) != RUNIT_OK) return st;
+        const uint32_t grid = min((uint32_t)ctx->sm_count, kMaxWorkers / kWarps);
+        runit_launch_chain_smem(ctx, paged_split_kernel<T, HD>, dim3(grid), dim3(kWarps * 32), smem, mk, mv, a, c.e0, c.n_entries);
+        if ((st = runit_after_launch(ctx, "paged_attention")) != RUNIT_OK) return st;
+        share = grid * kWarps / max(1u, c.n_entries * g->kv_heads);
     }
-    CUtensorMap mk, mv;
-    int32_t st = encode(ctx, g, g->k_pages, &mk);
-    if (st == RUNIT_OK) st = encode(ctx, g, g->v_pages, &mv);
-    if (st != RUNIT_OK) return st;
-    const uint32_t grid = min((uint32_t)ctx->sm_count, kMaxWorkers / kWarps), n_entries = b->n_seqs + (b->shared_len ? 1 : 0);
-    runit_launch_chain_smem(ctx, paged_split_kernel<T, HD>, dim3(grid), dim3(kWarps * 32), smem, mk, mv, a, n_entries);
-    if ((st = runit_after_launch(ctx, "paged_attention")) != RUNIT_OK) return st;
-    // warps of a merging block: about as many as a segment has pieces when all are alike
-    const uint32_t share = grid * kWarps / max(1u, b->n_seqs * g->kv_heads), warps = share >= 8 ? 8 : share >= 2 ? 4 : 1;
-    runit_launch_chain(ctx, merge_kernel<T, HD>, dim3(g->heads * b->rows), dim3(32 * warps), a, n_entries);
+    if (c.direct) return RUNIT_OK;
+    // warps of a merging block: about a quarter of the pieces that a segment has when all are alike
+    const uint32_t warps = share >= 32 ? 16 : share >= 16 ? 8 : share >= 4 ? 4 : 1;
+    const MergeArgs m{c.n_entries, c.own_tc ? c.own_split : 0, c.pre_tc ? c.pre_split : 0, own.part_o, own.part_ml, pre.part_o, pre.part_ml, b->shared_len != 0};
+    runit_launch_chain(ctx, merge_kernel<T, HD>, dim3(g->heads * b->rows), dim3(32 * warps), a, m);
     return runit_after_launch(ctx, "paged_attention (merge)");
 }
 
@@ -604,7 +716,7 @@ using namespace runit;
 extern "C" {
 
 size_t runit_paged_attention_scratch_bytes(const runit_paged_cfg* cfg, const runit_paged_batch* batch) {
-    return pg::why_not(cfg, batch) ? 0 : pg::layout_of(cfg, batch).bytes;
+    return pg::why_not(cfg, batch) ? 0 : pg::layout_of(cfg, batch, pg::choose(cfg, batch)).bytes;
 }
 
 int32_t runit_paged_attention(runit_ctx_t* ctx, const runit_paged_cfg* cfg, const runit_paged_batch* batch, const void* q, uint32_t ldq, void* out,
@@ -617,13 +729,14 @@ int32_t runit_paged_attention(runit_ctx_t* ctx, const runit_paged_cfg* cfg, cons
     RUNIT_REQUIRE(ctx, ldq % 8 == 0 && ldo % 8 == 0 && ldq >= (uint64_t)cfg->heads * cfg->dim && ldo >= (uint64_t)cfg->heads * cfg->dim,
                   "paged_attention: ldq=%u, ldo=%u must be multiples of 8, rows of heads * dim at least", ldq, ldo);
     RUNIT_REQUIRE(ctx, scratch && runit_aligned(scratch, 256), "paged_attention: scratch must be 256-byte aligned");
-    const pg::Layout l = pg::layout_of(cfg, batch);
+    const pg::Choice c = pg::choose(cfg, batch);
+    const pg::Layout l = pg::layout_of(cfg, batch, c);
     if (scratch_bytes < l.bytes) return runit_fail(ctx, RUNIT_ERR_BUFFER_SIZE, "paged_attention: %zu bytes of scratch, %zu needed", scratch_bytes, l.bytes);
     uint8_t* const s = (uint8_t*)scratch;
     const pg::AttnArgs a{pg::cache_of(ctx, cfg, batch), q, out, (const float*)cfg->slopes, ldq, ldo, cfg->window, cfg->scale, cfg->cap, (uint32_t*)(s + l.plan),
                          (float*)(s + l.slot_o), (float*)(s + l.slot_ml), (float*)(s + l.row_o), (float*)(s + l.row_ml), (float*)(s + l.pre_o), (float*)(s + l.pre_ml)};
-    if (cfg->type == RUNIT_TYPE_F16) return cfg->dim == 128 ? pg::run<__half, 128>(ctx, cfg, batch, a) : pg::run<__half, 64>(ctx, cfg, batch, a);
-    return cfg->dim == 128 ? pg::run<__nv_bfloat16, 128>(ctx, cfg, batch, a) : pg::run<__nv_bfloat16, 64>(ctx, cfg, batch, a);
+    if (cfg->type == RUNIT_TYPE_F16) return cfg->dim == 128 ? pg::run<__half, 128>(ctx, cfg, batch, a, c, s, l) : pg::run<__half, 64>(ctx, cfg, batch, a, c, s, l);
+    return cfg->dim == 128 ? pg::run<__nv_bfloat16, 128>(ctx, cfg, batch, a, c, s, l) : pg::run<__nv_bfloat16, 64>(ctx, cfg, batch, a, c, s, l);
 }
 
 }  // extern "C"

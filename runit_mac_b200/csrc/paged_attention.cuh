@@ -22,8 +22,15 @@ struct AttnArgs {
     uint32_t* plan;          // kPlanHead words, then the steps in front of every entry
     float *slot_o, *slot_ml; // [2 * workers][16][dim] and [..][16][2]: pieces of segments that workers share
     float *row_o, *row_ml;   // [rows * heads][dim] and [..][2]: what one worker has of a row whose shared positions come from elsewhere
-    float *pre_o, *pre_ml;   // the same for the shared positions (as many times as they are split)
+    float *pre_o, *pre_ml;   // the same for the shared positions
 };
+// What a launch of the kernel for many rows does (paged_attention_tc.cu): the shared positions for all rows, or every sequence's own positions.
+struct TcArgs {
+    uint32_t box, split;     // positions of a copy; parts that a tile's positions are cut into
+    bool shared, direct;     // direct: a row is done with this launch
+    float *part_o, *part_ml; // [split][rows * heads][dim] and [..][2]
+};
+int32_t paged_attention_tc(runit_ctx* ctx, const runit_paged_cfg* g, const AttnArgs& a, TcArgs w, uint32_t tiles);
 
 __device__ __forceinline__ float exp2_approx(float v) {
     float r;
@@ -73,6 +80,29 @@ template <> struct Half2<__nv_bfloat16> {
 // the 16-bit halves of w that are no numbers, set to zero
 template <typename T> __device__ __forceinline__ uint32_t finite_part(uint32_t w, uint32_t nf) { return w & ~((nf >> 15) * 0xFFFFu); }
 
+// cap * tanh(scale v / cap) of N products, for a whole warp.  Below 0.35 tanh u = u (1 - u^2/3 + 2 u^4/15 - 17 u^6/315 + 62 u^8/2835), its Taylor series,
+// whose next term is 2.4e-7 of u there; a warp with a larger argument takes (1 - e^-2|u|) / (1 + e^-2|u|), off by some 2^-22 of the cap.
+template <int N> __device__ __forceinline__ void cap_scores(float (&v)[N], float scale, float cap, float inv_cap) {
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        v[i] *= scale;
+        most = fmaxf(most, fabsf(v[i]));
+    }
+    if (__any_sync(0xffffffffu, most > 0.35f * cap)) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float e = exp2_approx(-2.f * kLog2e * fabsf(v[i]) * inv_cap);
+            v[i] = copysignf(cap * __fdividef(1.f - e, 1.f + e), v[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float u = v[i] * inv_cap, w = u * u;
+            v[i] *= fmaf(w, fmaf(w, fmaf(w, fmaf(w, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+        }
+    }
+}
 // The first position that the one at `pos` sees.
 __device__ __forceinline__ uint32_t first_seen(int32_t pos, uint32_t window) { return window && pos >= 0 && (uint32_t)pos >= window ? (uint32_t)pos + 1 - window : 0; }
 // Sequence of a row by halving the starts; c.n_seqs: nobody's.

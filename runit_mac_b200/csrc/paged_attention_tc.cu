@@ -1,0 +1,455 @@
+// Attention over a paged cache for many rows that share keys (prompts, and a prefix that a whole batch shares), on the tcgen05 tensor cores.
+//
+// A CTA has up to 256 (row, query head) pairs of one key head, as two tiles of 128, and walks a part of their positions in blocks of 128 that both tiles
+// share.  A tile's block: S = Q K^T into tensor memory (f32); four warps, a thread a row, take S into registers, form the weights 2^(s - ref), put
+// them down as 16-bit numbers in the columns of S; O += P V, accumulated in tensor memory, P being the A operand from there and V (as it lies in the cache)
+// MN-major.  The products of one tile run under the exponentials of the other.  ref is a row's largest score until one exceeds it by 2^8, so that O
+// is rarely scaled; weights up to 2^8 keep the relative error of their rounding, and sums of them are f32.
+// Bound: exponentials (16 a clock and SM) and products (4096 multiply-adds a clock and SM) both take 2048 clocks for 256 rows x 128 positions x dim 128.
+// K and V of a block come by TMA as boxes of whole pages or of 128 positions; positions outside of what the CTA's rows see are zeros in V.
+#include "paged_attention.cuh"
+#include "tcgen05.cuh"
+
+namespace runit {
+namespace pg {
+
+constexpr uint32_t kTcRows = 256, kKeys = 128, kSoftWarps = 8, kTcThreads = 32 * (kSoftWarps + 2);
+constexpr float kRise = 8.f;                       // log2 of what a weight may exceed 1 by
+
+template <int HD> struct TcShape {
+    static constexpr uint32_t kPanel = 128 * 128;  // 64 elements of 128 rows
+    static constexpr uint32_t kTile = HD / 64 * kPanel;
+    static constexpr uint32_t kSlots = HD == 128 ? 5 : 10;      // of K and V blocks in turn
+    static constexpr uint32_t kSmem = (2 + kSlots) * kTile + 1024;
+};
+
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, uint32_t panel) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+template <typename T> __host__ __device__ constexpr uint32_t idesc_of(uint32_t m, uint32_t n, uint32_t b_mn);
+template <> __host__ __device__ constexpr uint32_t idesc_of<__half>(uint32_t m, uint32_t n, uint32_t b_mn) { return umma_idesc_f16(m, n, b_mn); }
+template <> __host__ __device__ constexpr uint32_t idesc_of<__nv_bfloat16>(uint32_t m, uint32_t n, uint32_t b_mn) { return umma_idesc_f16(m, n, b_mn) | (1u << 7) | (1u << 10); }
+
+// One row's attention over positions lo .. hi of a table, by a warp with plain arithmetic: for rows whose products met a value that is no number at a
+// position that they do not see (0 x Inf).  Returns maximum (log2 units) and sum; o: HD / 32 of the dimensions per lane.
+template <typename T, int HD>
+__device__ __noinline__ float2 plain_row(const AttnArgs& a, const int32_t* table, uint32_t token, uint32_t head, int32_t pos, uint32_t lo, uint32_t hi, float* out) {
+    constexpr uint32_t E = HD / 32;
+    const Cache& c = a.c;
+    const uint32_t lane = threadIdx.x & 31;
+    const T* qp = reinterpret_cast<const T*>(a.q) + (size_t)token * a.ldq + (size_t)head * HD + lane * E;
+    float x[E], o[E], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (uint32_t e = 0; e < E; e++) { x[e] = to_f32(qp[e]); o[e] = 0.f; }
+    const float slope = a.slopes ? a.slopes[head] : 0.f;
+    for (uint32_t j = lo; j < hi; j++) {
+        bool ok;
+        const size_t at = page_row(c, table, j, head / c.group, &ok) + lane * E;
+        float t = 0.f;
+#pragma unroll
+        for (uint32_t e = 0; e < E; e++) t = fmaf(x[e], to_f32(reinterpret_cast<const T*>(c.k)[at + e]), t);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
+        t *= a.scale;
+        if (a.cap != 0.f) t = a.cap * tanhf(t / a.cap);
+        t = (t - slope * (float)(pos - (int32_t)j)) * kLog2e;
+        const float top = fmaxf(m, t), old = top == -INFINITY ? 1.f : exp2_approx(m - top), p = exp2_approx(top == -INFINITY ? t : t - top);
+        l = fmaf(l, old, p);
+#pragma unroll
+        for (uint32_t e = 0; e < E; e++) o[e] = fmaf(o[e], old, p * to_f32(reinterpret_cast<const T*>(c.v)[at + e]));
+        m = top;
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < E; e++) out[e] = o[e];
+    return make_float2(m, l);
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const AttnArgs a, const TcArgs w) {
+    using S = TcShape<HD>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * S::kSlots + 6];
+    __shared__ uint32_t tmem_holder, found[4], sums[kTcThreads / 32];
+    __shared__ volatile int abort_flag;
+    const Cache& c = a.c;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    // full, empty: one phase per use of a slot; s_full, p_full: one per block of a tile; done: one
+    const uint32_t full = smem_u32(bars), empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots, p_full = s_full + 16, done = p_full + 16;
+    if (tid == 0) {
+        abort_flag = 0;
+        for (uint32_t i = 0; i < 2 * S::kSlots + 6; i++) mbar_init(full + 8 * i, i >= 2 * S::kSlots + 2 && i < 2 * S::kSlots + 4 ? 128 : 1);
+        fence_mbar_init();
+        found[0] = 0xFFFFFFFFu;
+        found[2] = c.shared;
+        found[3] = 0;
+    }
+    if (warp == 0) {
+        tmem_alloc(smem_u32(&tmem_holder), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = tmem_holder;
+    grid_dependency_wait();
+    grid_launch_dependents();
+
+    // which rows and positions
+    const uint32_t part = blockIdx.x % w.split, h = blockIdx.x / w.split % c.kv_heads, index = blockIdx.x / w.split / c.kv_heads;
+    if (w.shared) {
+        uint32_t lo = c.shared, hi = 0;
+        for (uint32_t e = tid; e < c.n_seqs; e += kTcThreads) {
+            const Seq s = sequence(c, e);
+            if (!s.n) continue;
+            lo = min(lo, first_seen((int32_t)s.len - (int32_t)s.n, a.window));
+            hi = max(hi, min(s.len, c.shared));
+        }
+        atomicMin(&found[2], lo);
+        atomicMax(&found[3], hi);
+        if (tid == 0) {
+            found[0] = c.n_seqs;
+            found[1] = index;
+        }
+    } else {                                   // tiles in front of a sequence; the last ones (those with the most positions) begin
+        const uint32_t per = (c.n_seqs + kTcThreads - 1) / kTcThreads, beg = min(c.n_seqs, tid * per), end = min(c.n_seqs, beg + per);
+        uint32_t sum = 0;
+        for (uint32_t e = beg; e < end; e++) sum += (sequence(c, e).n * c.group + kTcRows - 1) / kTcRows;
+        uint32_t inc = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= (uint32_t)o) inc += v;
+        }
+        if (lane == 31) sums[warp] = inc;
+        __syncthreads();
+        uint32_t off = inc - sum, total = 0;
+        for (uint32_t i = 0; i < kTcThreads / 32; i++) {
+            if (i < warp) off += sums[i];
+            total += sums[i];
+        }
+        const uint32_t want = total - 1 - index;                 // beyond every tile where index >= total
+        if (index < total && want >= off && want < off + sum) {
+            uint32_t e = beg, at = off;
+            for (;; e++) {
+                const uint32_t n = (sequence(c, e).n * c.group + kTcRows - 1) / kTcRows;
+                if (want < at + n) break;
+                at += n;
+            }
+            found[0] = e;
+            found[1] = want - at;
+        }
+    }
+    __syncthreads();
+    const uint32_t entry = found[0], tile = found[1];
+    uint32_t row0 = 0, n_pairs = c.rows * c.group, lo = 0, hi = 0;
+    int32_t base_pos = 0;
+    const int32_t* table = c.table;
+    if (w.shared) {
+        lo = found[2];
+        hi = found[3];
+    } else if (entry != 0xFFFFFFFFu) {
+        const Seq s = sequence(c, entry);
+        row0 = s.row0;
+        n_pairs = s.n * c.group;
+        base_pos = (int32_t)s.len - (int32_t)s.n;
+        const uint32_t last = min(n_pairs, (tile + 1) * kTcRows) - 1;
+        lo = max(c.shared, first_seen(base_pos + (int32_t)(tile * kTcRows / c.group), a.window));
+        hi = (uint32_t)max(0, base_pos + (int32_t)(last / c.group) + 1);
+        table += (size_t)entry * c.table_ld;
+    }
+    const bool any = entry != 0xFFFFFFFFu && tile * kTcRows < n_pairs;
+    const uint32_t first_row = tile * kTcRows, start = lo & ~(w.box - 1), steps = any && hi > lo ? (hi - start + kKeys - 1) / kKeys : 0;
+    const uint32_t b0 = (uint32_t)((uint64_t)part * steps / w.split), n_blocks = (uint32_t)((uint64_t)(part + 1) * steps / w.split) - b0;
+    const uint32_t chains = any && n_pairs - first_row > 128 ? 2 : 1;
+    bool ok = true;
+
+    if (warp == kSoftWarps + 1) {              // copies: K(0), V(0), K(1), ... into the slots in turn
+        uint32_t n = 0;
+        const uint32_t boxes = kKeys / w.box;
+        for (uint32_t j = 0; j < n_blocks && ok; j++) {
+            const uint32_t k0 = start + (b0 + j) * kKeys, k = k0 + lane * w.box;
+            const bool mine = lane < boxes && k < hi && k + w.box > lo;
+            int32_t page = mine ? table[k >> c.page_log2] : 0;
+            if ((uint32_t)page >= c.n_pages) {
+                report(c);
+                page = 0;
+            }
+            const int32_t row = (int32_t)((((uint32_t)page * c.kv_heads + h) << c.page_log2) + (k & ((1u << c.page_log2) - 1)));
+            const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * w.box * HD * 2;
+            for (uint32_t v = 0; v < 2 && ok; v++, n++) {
+                const uint32_t slot = n % S::kSlots, bar = full + 8 * slot, dst = base + (2 + slot) * S::kTile;
+                if (n >= S::kSlots) ok = mbar_wait_timed(empty + 8 * slot, (n / S::kSlots - 1) & 1, &abort_flag);
+                if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                if (lane == 0) mbar_expect_tx(bar, bytes);
+                __syncwarp();
+                if (mine)
+                    for (uint32_t p = 0; p < HD / 64; p++) tma_load_2d(dst + p * S::kPanel + lane * w.box * 128, v ? &mv : &mk, 128 * p, row, bar);
+                __syncwarp();
+            }
+        }
+        // nothing is in flight when the block leaves
+        mbar_drain(full, S::kSlots, n);
+    } else if (warp == kSoftWarps) {           // products
+        uint32_t n_s[2] = {0, 0}, n_d[2] = {0, 0};
+        auto q_tile = [&](uint32_t i) { return base + i * S::kTile; };
+        auto slot_of_use = [&](uint32_t n) { return base + (2 + n % S::kSlots) * S::kTile; };
+        auto wait_full = [&](uint32_t n) {
+            ok = ok && mbar_wait_timed(full + 8 * (n % S::kSlots), (n / S::kSlots) & 1, &abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after_sync();
+        };
+        auto scores = [&](uint32_t i, uint32_t kb) {
+            if (elect_one()) {
+#pragma unroll
+                for (int s = 0; s < HD / 16; s++) {
+                    const uint32_t off = (s >> 2) * S::kPanel + (s & 3) * 32;
+                    umma_bf16(tmem + 128 * i, umma_desc_sw128(q_tile(i) + off), umma_desc_sw128(kb + off), idesc_of<T>(128, kKeys, 0), s > 0);
+                }
+                umma_commit(s_full + 8 * i);
+            }
+            __syncwarp();
+            n_s[i]++;
+        };
+        asm volatile("bar.sync 1, 288;" ::: "memory");           // Q is there
+        tc_fence_after_sync();
+        if (n_blocks > 0) {
+            wait_full(0);
+            for (uint32_t i = 0; i < chains && ok; i++) scores(i, slot_of_use(0));
+            if (ok && elect_one()) umma_commit(empty);
+            __syncwarp();
+        }
+        for (uint32_t j = 0; j < n_blocks && ok; j++) {
+            const bool last = j + 1 == n_blocks;
+            const uint32_t uv = 2 * j + 1, uk = 2 * j + 2, k0 = start + (b0 + j) * kKeys, vb = slot_of_use(uv);
+            wait_full(uv);
+            if (!ok) break;
+            if (k0 < lo || k0 + kKeys > hi) {  // zeros where no row looks: the copies have left there what lay there, or the neighbours of what was asked for
+                const uint32_t from = lo > k0 ? lo - k0 : 0, to = hi - k0;
+                for (uint32_t x = lane; x < kKeys * (HD / 8); x += 32) {
+                    const uint32_t r = x / (HD / 8), ch = x % (HD / 8);
+                    if (r >= from && r < to) continue;
+                    *reinterpret_cast<uint4*>(smem_raw + (vb - smem_u32(smem_raw)) + (ch >> 3) * S::kPanel + r * 128 + ((ch & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async();
+                __syncwarp();
+            }
+            for (uint32_t i = 0; i < chains && ok; i++) {
+                ok = mbar_wait_timed(p_full + 8 * i, j & 1, &abort_flag);
+                if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                tc_fence_after_sync();
+                if (elect_one()) {
+#pragma unroll
+                    for (int s = 0; s < (int)kKeys / 16; s++)
+                        umma_f16_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * s, desc_mn_sw128(vb + s * 2048, S::kPanel), idesc_of<T>(128, HD, 1), j > 0 || s > 0);
+                    if (last) umma_commit(done + 8 * i);
+                    else if (i + 1 == chains) umma_commit(empty + 8 * (uv % S::kSlots));
+                }
+                __syncwarp();
+                if (last) {
+                    n_d[i]++;
+                    continue;
+                }
+                if (i == 0) wait_full(uk);
+                if (ok) scores(i, slot_of_use(uk));
+            }
+            if (!last && ok) {
+                if (elect_one()) umma_commit(empty + 8 * (uk % S::kSlots));
+                __syncwarp();
+            }
+        }
+        for (uint32_t i = 0; i < chains; i++) {                  // nor is a product when the tensor memory goes back
+            mbar_drain(s_full + 8 * i, 1, n_s[i]);
+            mbar_drain(done + 8 * i, 1, n_d[i]);
+        }
+    } else {
+        const uint32_t chain = warp >> 2, row = tid & 127, pair = first_row + chain * 128 + row;
+        const uint32_t lanes = (warp & 3) << 21, s_cols = tmem + 128 * chain + lanes, o_cols = tmem + 256 + 128 * chain + lanes;
+        bool live = any && pair < n_pairs;
+        const uint32_t token = row0 + (live ? pair / c.group : 0), head = h * c.group + (live ? pair % c.group : 0);
+        int32_t pos = base_pos + (int32_t)(pair / c.group);
+        uint32_t limit = 0x7FFFFFFFu;
+        if (w.shared && live) {
+            const uint32_t s = sequence_by_halves(c, token);
+            live = s < c.n_seqs;
+            if (live) {
+                const Seq q = sequence(c, s);
+                live = token >= q.row0 && token < q.row0 + q.n;
+                pos = (int32_t)q.len - (int32_t)(q.row0 + q.n - token);
+            }
+            limit = c.shared;
+        }
+        const uint32_t row_lo = !live ? 0 : max(w.shared ? 0 : c.shared, first_seen(pos, a.window)), row_hi = !live ? 0x7FFFFFFFu : min((uint32_t)max(0, pos + 1), limit);
+        const float slope = a.slopes && live ? a.slopes[head] : 0.f;
+        {
+            const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (size_t)token * a.ldq + (size_t)head * HD);
+            uint8_t* dst = smem_raw + (base - smem_u32(smem_raw)) + chain * S::kTile + row * 128;
+#pragma unroll
+            for (uint32_t ch = 0; ch < HD / 8; ch++)
+                *reinterpret_cast<uint4*>(dst + (ch >> 3) * S::kPanel + (((ch & 7) ^ (row & 7)) << 4)) = live ? src[ch] : make_uint4(0, 0, 0, 0);
+            fence_proxy_async();
+        }
+        asm volatile("bar.sync 1, 288;" ::: "memory");
+        const bool plain = a.cap == 0.f && !a.slopes && a.scale > 0.f;
+        const float mul = plain ? a.scale * kLog2e : kLog2e, pre = a.cap != 0.f ? 1.f : a.scale, inv_cap = a.cap != 0.f ? 1.f / a.cap : 0.f;
+        float ref = -INFINITY, l = 0.f;
+        bool cut = false;                      // some block had positions that this row does not see
+        if (chain < chains) {
+            for (uint32_t j = 0; j < n_blocks; j++) {
+                if (ok) ok = mbar_wait_timed(s_full + 8 * chain, j & 1, &abort_flag);
+                __syncwarp();
+                tc_fence_after_sync();
+                const uint32_t k0 = start + (b0 + j) * kKeys;
+                uint32_t r[4][32];
+#pragma unroll
+                for (int q = 0; q < 4; q++) tmem_ld32(s_cols + 32 * q, r[q]);
+                tmem_ld_wait();
+                const bool inside = k0 >= row_lo && k0 + kKeys <= row_hi;
+                cut |= !inside;
+                if (!__all_sync(0xffffffffu, plain && inside)) {
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        if (a.cap != 0.f) cap_scores(reinterpret_cast<float(&)[32]>(r[q]), a.scale, a.cap, inv_cap);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) {
+                            const uint32_t key = k0 + 32 * q + e;
+                            float v = __uint_as_float(r[q][e]);
+                            if (!plain) v = v * pre - slope * (float)(pos - (int32_t)key);
+                            if (key < row_lo || key >= row_hi) v = -INFINITY;
+                            r[q][e] = __float_as_uint(v);
+                        }
+                    }
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) mx[q] = fmaxf(mx[q], fmaxf(__uint_as_float(r[q][e]), __uint_as_float(r[q][e + 1])));
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
+                const bool rise = top > ref + kRise || (ref == -INFINITY && top > ref);
+                const float corr = rise ? exp2_approx(ref - top) : 1.f;
+                l *= corr;
+                ref = rise ? top : ref;
+                // S of this block comes behind the product of the last one: O is complete
+                if (__any_sync(0xffffffffu, rise) && j > 0) {
+#pragma unroll 1
+                    for (int q = 0; q < HD / 16; q++) {
+                        uint32_t o[16];
+                        tmem_ld16(o_cols + 16 * q, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                        tmem_st16(o_cols + 16 * q, o);
+                    }
+                }
+                const float sub = ref == -INFINITY ? 0.f : ref;
+                const uint64_t mul2 = packf(mul), sub2 = packf(-sub);
+                uint64_t both = 0;
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    uint32_t p[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const uint64_t x = ffma2(pack2(r[q][2 * e], r[q][2 * e + 1]), mul2, sub2);
+                        const float p0 = exp2_approx(__uint_as_float((uint32_t)x)), p1 = exp2_approx(__uint_as_float((uint32_t)(x >> 32)));
+                        both = fadd2(both, pack2(__float_as_uint(p0), __float_as_uint(p1)));
+                        // the weights meet the values in the cache's type: half a step of it, relative, each; their sum is that of the 32-bit ones
+                        p[e] = Half2<T>::pack(p0, p1);
+                    }
+                    tmem_st16(s_cols + 16 * q, p);
+                }
+                l += sum2(both);
+                tmem_st_wait();
+                tc_fence_before_sync();
+                mbar_arrive(p_full + 8 * chain);
+            }
+            if (n_blocks > 0 && ok) ok = mbar_wait_timed(done + 8 * chain, 0, &abort_flag);
+            __syncwarp();
+            tc_fence_after_sync();
+            // the row's result: final, or this part's sums
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const size_t orow = (size_t)token * c.heads + head;
+            float* po = w.part_o + ((size_t)part * c.rows * c.heads + orow) * HD;
+            float* pml = w.part_ml + ((size_t)part * c.rows * c.heads + orow) * 2;
+            T* dst = reinterpret_cast<T*>(a.out) + (size_t)token * a.ldo + (size_t)head * HD;
+            bool odd = false;
+#pragma unroll 1
+            for (int q = 0; q < HD / 32; q++) {
+                uint32_t o[32];
+                if (n_blocks > 0) {
+                    tmem_ld32(o_cols + 32 * q, o);
+                    tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = 0;
+                }
+                if (!live || !ok) continue;
+#pragma unroll
+                for (int e = 0; e < 32; e++) odd |= !(fabsf(__uint_as_float(o[e])) < INFINITY);
+                if (w.direct) {
+                    uint32_t x[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[e] = Half2<T>::pack(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) reinterpret_cast<uint4*>(dst + 32 * q)[e] = make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) reinterpret_cast<uint4*>(po + 32 * q)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                }
+            }
+            if (live && ok && !w.direct) *reinterpret_cast<float2*>(pml) = make_float2(ref, l);
+            uint32_t again = __ballot_sync(0xffffffffu, live && ok && odd && cut);
+            while (again) {
+                const uint32_t from = __ffs(again) - 1;
+                again &= again - 1;
+                const uint32_t tk = __shfl_sync(0xffffffffu, token, from), hd = __shfl_sync(0xffffffffu, head, from);
+                const uint32_t k_lo = max(__shfl_sync(0xffffffffu, row_lo, from), start + b0 * kKeys), k_hi = min(__shfl_sync(0xffffffffu, row_hi, from), start + (b0 + n_blocks) * kKeys);
+                float x[HD / 32];
+                const float2 ml = plain_row<T, HD>(a, table, tk, hd, __shfl_sync(0xffffffffu, pos, from), k_lo, k_hi, x);
+                const size_t at = (size_t)tk * c.heads + hd;
+                const float f = w.direct ? (ml.y == 0.f ? 0.f : 1.f / ml.y) : 1.f;
+                for (uint32_t e = 0; e < HD / 32; e++) {
+                    const uint32_t d = lane * (HD / 32) + e;
+                    if (w.direct) (reinterpret_cast<T*>(a.out) + (size_t)tk * a.ldo + (size_t)hd * HD)[d] = from_f32<T>(x[e] * f);
+                    else w.part_o[((size_t)part * c.rows * c.heads + at) * HD + d] = x[e];
+                }
+                if (!w.direct && lane == 0) *reinterpret_cast<float2*>(w.part_ml + ((size_t)part * c.rows * c.heads + at) * 2) = ml;
+                __syncwarp();
+            }
+        }
+    }
+    if (!ok) {
+        abort_flag = 1;
+        if (c.status) atomicCAS(c.status, 0, 1);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <typename T, int HD>
+static int32_t run_tc(runit_ctx* ctx, const runit_paged_cfg* g, const AttnArgs& a, TcArgs w, uint32_t tiles) {
+    static bool configured[64] = {false};
+    if (ctx->device >= 64 || !configured[ctx->device]) {
+        RUNIT_CUDA_TRY(ctx, cudaFuncSetAttribute(attention_tc_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<HD>::kSmem));
+        if (ctx->device < 64) configured[ctx->device] = true;
+    }
+    CUtensorMap m[2];
+    for (int i = 0; i < 2; i++) {
+        const int32_t st = runit_get_tmap(ctx, i ? g->v_pages : g->k_pages, (uint64_t)g->n_pages * g->kv_heads * g->page, HD * 2, w.box, 128, &m[i], 1);
+        if (st != RUNIT_OK) return st;
+    }
+    runit_launch_chain_smem(ctx, attention_tc_kernel<T, HD>, dim3(tiles * g->kv_heads * w.split), dim3(kTcThreads), TcShape<HD>::kSmem, m[0], m[1], a, w);
+    return runit_after_launch(ctx, "paged_attention (many rows)");
+}
+
+int32_t paged_attention_tc(runit_ctx* ctx, const runit_paged_cfg* g, const AttnArgs& a, TcArgs w, uint32_t tiles) {
+    if (g->type == RUNIT_TYPE_F16) return g->dim == 128 ? run_tc<__half, 128>(ctx, g, a, w, tiles) : run_tc<__half, 64>(ctx, g, a, w, tiles);
+    return g->dim == 128 ? run_tc<__nv_bfloat16, 128>(ctx, g, a, w, tiles) : run_tc<__nv_bfloat16, 64>(ctx, g, a, w, tiles);
+}
+
+}  // namespace pg
+}  // namespace runit
