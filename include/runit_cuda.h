@@ -655,7 +655,7 @@ int32_t runit_paged_attention(runit_ctx_t*, const runit_paged_cfg* cfg, const ru
 /* Rows of n logits (type f32, f16 or bf16; ld elements apart): logprob f32 [rows] = log softmax at tokens[row] (int32; 0 for a token outside 0 .. n - 1,
  * which marks a row without one; tokens and logprob may both be NULL), entropy f32 [rows] of the softmax (may be NULL), and its k most probable entries
  * (k <= 32 and k <= n): top_ids int32 [rows][k], descending, equal logits by index, and top_logprobs f32 [rows][k] (both NULL with k = 0).  A NaN counts as
- * the largest logit and makes the row's values NaN; in a row of -Inf alone every log probability is -Inf and the entropy 0. */
+ * the largest logit and makes the row's values NaN, and so does +Inf; in a row of -Inf alone every log probability is -Inf and the entropy 0. */
 int32_t runit_token_logprobs(runit_ctx_t*, const void* logits, int32_t type, uint32_t ld, uint32_t n, uint32_t rows, const void* tokens, void* logprob,
                              void* entropy, uint32_t k, void* top_ids, void* top_logprobs);
 
