@@ -86,15 +86,30 @@ __device__ __forceinline__ void join(Top& t, const Top& o) {
     }
 }
 
+constexpr float kFloor = -1e38f;               // -Inf in the fast path, where the maximum is above kLow, so far above that the floor has no mass
+
+// Sixteen bytes of logits: unpacked; their maximum (a NaN stays one); unpacked with -Inf raised to the floor (f16: to its lowest number).
 template <typename T> struct Vec;
 template <> struct Vec<float> {
     static constexpr uint32_t N = 4;
+    static constexpr float kLow = -1e37f;
     static __device__ __forceinline__ void unpack(const uint4& u, float (&v)[4]) {
         v[0] = __uint_as_float(u.x); v[1] = __uint_as_float(u.y); v[2] = __uint_as_float(u.z); v[3] = __uint_as_float(u.w);
     }
+    static __device__ __forceinline__ float most(const uint4& u) {
+        return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)), max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
+    }
+    static __device__ __forceinline__ void raised(const uint4& u, float (&v)[4]) {
+        unpack(u, v);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = fmaxf(v[i], kFloor);
+    }
+    static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u); }
+    static __device__ __forceinline__ uint4 one(float v) { return make_uint4(__float_as_uint(v), 0xFF800000u, 0xFF800000u, 0xFF800000u); }
 };
 template <> struct Vec<__half> {
     static constexpr uint32_t N = 8;
+    static constexpr float kLow = -6e4f;
     static __device__ __forceinline__ void unpack(const uint4& u, float (&v)[8]) {
         const __half2* h = reinterpret_cast<const __half2*>(&u);
 #pragma unroll
@@ -104,9 +119,24 @@ template <> struct Vec<__half> {
             v[2 * i + 1] = f.y;
         }
     }
+    static __device__ __forceinline__ float most(const uint4& u) {
+        const __half2* h = reinterpret_cast<const __half2*>(&u);
+        const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+        return max_nan(__low2float(m), __high2float(m));
+    }
+    static __device__ __forceinline__ void raised(const uint4& u, float (&v)[8]) {
+        uint4 r;
+        const __half2 low = __half2half2(__ushort_as_half(0xFBFF));
+#pragma unroll
+        for (int i = 0; i < 4; i++) reinterpret_cast<__half2*>(&r)[i] = __hmax2(reinterpret_cast<const __half2*>(&u)[i], low);
+        unpack(r, v);
+    }
+    static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u); }
+    static __device__ __forceinline__ uint4 one(__half v) { return make_uint4(0xFC000000u | __half_as_ushort(v), 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u); }
 };
 template <> struct Vec<__nv_bfloat16> {
     static constexpr uint32_t N = 8;
+    static constexpr float kLow = -1e37f;
     static __device__ __forceinline__ void unpack(const uint4& u, float (&v)[8]) {
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -115,70 +145,85 @@ template <> struct Vec<__nv_bfloat16> {
             v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
         }
     }
+    static __device__ __forceinline__ float most(const uint4& u) {
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+        const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+        return max_nan(__low2float(m), __high2float(m));
+    }
+    static __device__ __forceinline__ void raised(const uint4& u, float (&v)[8]) {
+        uint4 r;
+        const __nv_bfloat162 low = __bfloat162bfloat162(__ushort_as_bfloat16(0xFE96));           // -1e38
+#pragma unroll
+        for (int i = 0; i < 4; i++) reinterpret_cast<__nv_bfloat162*>(&r)[i] = __hmax2(reinterpret_cast<const __nv_bfloat162*>(&u)[i], low);
+        unpack(r, v);
+    }
+    static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u); }
+    static __device__ __forceinline__ uint4 one(__nv_bfloat16 v) { return make_uint4(0xFF800000u | __bfloat16_as_ushort(v), 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u); }
 };
 
-// A warp's pass over its share of a row, in the order of the indices.  The maximum is the warp's: it rises some ten times in a share, and then
-// only the sums are scaled; one lane leaves the maximal entry out.
-template <bool TOP, int N> struct Pass {
-    float m = -INFINITY;
-    uint32_t owner = 32;                       // the lane that has left an entry out
+// A warp's pass over its share of a row, in the order of the indices.  The maximum is the warp's: it rises some ten times in a share, and only
+// then are the sums scaled; one lane leaves the maximal entry out.
+template <typename T, bool TOP> struct Pass {
+    static constexpr uint32_t N = Vec<T>::N;
+    float m = -INFINITY, mine = -INFINITY;     // of the warp; of the lane's vectors
+    uint32_t owner = 32, at = 0xFFFFFFFFu;     // the lane that has left an entry out; the lane's first vector that has `mine`
     uint64_t z2 = 0, b2 = 0;
-    Top top = {0, 0};
-    float least = NAN;                         // the k-th so far: nothing is known of what is not above it.  NaN: fewer than k
-    uint32_t k;
 
-    __device__ __forceinline__ explicit Pass(uint32_t k_) : k(k_) {}
-    // entries i, i + 1, ...: `count` of them, the others of v are -Inf
-    __device__ __forceinline__ void take(const float (&v)[N], uint32_t i, uint32_t count) {
-        float most = v[0];
+    // vector i of the row (-Inf where there is nothing; `in`: it counts among the lane's)
+    __device__ __forceinline__ void take(const uint4& u, uint32_t i, bool in) {
+        const float most = Vec<T>::most(u);
+        const bool up = !(most <= m);
+        if (__any_sync(0xffffffffu, up || m < Vec<T>::kLow)) {
+            rise(u, most, i, in);
+            return;
+        }
+        if (TOP && most > mine && in) { mine = most; at = i; }
+        float v[N];
+        Vec<T>::raised(u, v);
+        const uint64_t sub2 = packf(-m), l2 = packf(kLog2e);
 #pragma unroll
-        for (int e = 1; e < N; e++) most = max_nan(most, v[e]);
+        for (uint32_t e = 0; e < N; e += 2) {
+            const uint64_t d = fadd2(pack2(__float_as_uint(v[e]), __float_as_uint(v[e + 1])), sub2), t = fmul2(d, l2);
+            const uint64_t p = pack2(__float_as_uint(exp2_approx(__uint_as_float((uint32_t)t))), __float_as_uint(exp2_approx(__uint_as_float((uint32_t)(t >> 32)))));
+            z2 = fadd2(z2, p);
+            b2 = ffma2(p, d, b2);
+        }
+    }
+    // the same where the maximum rises, is no number or is very low
+    __device__ __forceinline__ void rise(const uint4& u, float most, uint32_t i, bool in) {
+        const uint32_t lane = threadIdx.x & 31;
+        if (TOP && in && (most > mine || (most != most && mine == mine))) { mine = most; at = i; }
         bool leave = false;
         if (__any_sync(0xffffffffu, !(most <= m))) {
             float now = max_nan(m, most);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) now = max_nan(now, __shfl_xor_sync(0xffffffffu, now, o));
-            const uint32_t lane = threadIdx.x & 31;
             const float d = m == -INFINITY ? kLeast : m - now, w = m == -INFINITY ? 0.f : exp_of(d);
-            float z = sum2(z2), b = sum2(b2);
-            if (lane == owner) z += 1.f;       // what was left out so far
-            b = w * fmaf(d, z, b);
+            const float z = sum2(z2) + (lane == owner ? 1.f : 0.f), b = sum2(b2);         // with what was left out so far
             z2 = pack2(__float_as_uint(w * z), 0);
-            b2 = pack2(__float_as_uint(b), 0);
+            b2 = pack2(__float_as_uint(w * fmaf(d, z, b)), 0);
             m = now;
             owner = __ffs(__ballot_sync(0xffffffffu, most == now)) - 1;
             leave = lane == owner;
         }
         const float sub = m == -INFINITY ? 0.f : m;
-        const uint64_t sub2 = packf(-sub), l2 = packf(kLog2e);
+        float v[N], z = 0.f, b = 0.f;
+        Vec<T>::unpack(u, v);
 #pragma unroll
-        for (int e = 0; e < N; e += 2) {
-            uint64_t d = fadd2(pack2(__float_as_uint(v[e]), __float_as_uint(v[e + 1])), sub2);
-            d = pack2(__float_as_uint(fmaxf(__uint_as_float((uint32_t)d), kLeast)), __float_as_uint(fmaxf(__uint_as_float((uint32_t)(d >> 32)), kLeast)));
-            const uint64_t t = fmul2(d, l2);
-            float p0 = exp2_approx(__uint_as_float((uint32_t)t)), p1 = exp2_approx(__uint_as_float((uint32_t)(t >> 32)));
-            if (leave && v[e] == m) { p0 = 0.f; leave = false; }
-            if (leave && v[e + 1] == m) { p1 = 0.f; leave = false; }
-            const uint64_t p = pack2(__float_as_uint(p0), __float_as_uint(p1));
-            z2 = fadd2(z2, p);
-            b2 = ffma2(p, d, b2);
+        for (uint32_t e = 0; e < N; e++) {
+            const float d = fmaxf(v[e] - sub, kLeast);
+            float p = exp_of(d);
+            if (leave && v[e] == m) { p = 0.f; leave = false; }
+            z += p;
+            b = fmaf(p, d, b);
         }
-        if constexpr (TOP) {
-            bool open = count > 0;
-            uint32_t who;
-            while ((who = __ballot_sync(0xffffffffu, open && !(most <= least))) != 0) {
-                const uint32_t from = __ffs(who) - 1, n = __shfl_sync(0xffffffffu, count, from), i0 = __shfl_sync(0xffffffffu, i, from);
-                open = open && (threadIdx.x & 31) != from;
-#pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const float x = __shfl_sync(0xffffffffu, v[e], from);
-                    if ((uint32_t)e >= n || x <= least) continue;
-                    insert(top, order(x), ~(i0 + e));
-                    const uint32_t last = __shfl_sync(0xffffffffu, top.v, k - 1);
-                    least = last ? value(last) : NAN;
-                }
-            }
-        }
+        z2 = fadd2(z2, pack2(__float_as_uint(z), 0));
+        b2 = fadd2(b2, pack2(__float_as_uint(b), 0));
+    }
+    // the lane's largest entry; first: its first vector, if it has any
+    __device__ __forceinline__ Top top(uint32_t first, uint32_t end) const {
+        if (at != 0xFFFFFFFFu) return Top{order(mine), ~at};
+        return first < end ? Top{order(-INFINITY), ~first} : Top{0, 0};
     }
     __device__ __forceinline__ Sums sums() const {
         Sums s{m, sum2(z2), sum2(b2)};
@@ -194,6 +239,33 @@ template <bool TOP, int N> struct Pass {
     }
 };
 
+// The lists of a block's warps joined: the result in warp 0.  All threads.
+__device__ __forceinline__ void join_warps(Top& t, Top (*lists)[32]) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    lists[warp][lane] = t;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = kWarps / 2; w > 0; w /= 2) {
+        if (warp < w) {
+            join(t, lists[warp + w][lane]);
+            lists[warp][lane] = t;
+        }
+        __syncthreads();
+    }
+}
+// Descending order of the lanes' entries.
+__device__ __forceinline__ void sort_lanes(Top& t) {
+    const uint32_t lane = threadIdx.x & 31;
+#pragma unroll
+    for (uint32_t n = 2; n <= 32; n *= 2)
+#pragma unroll
+        for (uint32_t d = n / 2; d > 0; d /= 2) {
+            const uint32_t xv = __shfl_xor_sync(0xffffffffu, t.v, d), xi = __shfl_xor_sync(0xffffffffu, t.i, d);
+            const bool up = (lane & n) != 0;                     // this stretch ascends
+            if (before(t, xv, xi) == (((lane & d) != 0) != up) && (t.v != xv || t.i != xi)) { t.v = xv; t.i = xi; }
+        }
+}
+
 // A cluster of `cluster` blocks per row (a power of two up to 16), each with a run of the row; the first one adds up.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a, const uint32_t cluster) {
@@ -201,7 +273,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a, 
     grid_dependency_wait();
     grid_launch_dependents();
     __shared__ Sums part[kWarps], all;
-    __shared__ Top tops[kWarps][32], best[32];
+    __shared__ Top lists[kWarps][32], best[32];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.x / cluster, rank = blockIdx.x % cluster;
     const T* x = reinterpret_cast<const T*>(a.x) + (size_t)row * a.ld;
     // entries ahead of the first 16-byte boundary, whole vectors, entries behind the last
@@ -214,14 +286,9 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a, 
         token = a.tokens[row];
         if ((uint32_t)token < a.n) xt = to_f32(x[token]);
     }
-    Pass<TOP, N> pass(a.k);
-    float v[N];
-    auto few = [&](uint32_t first, uint32_t count) {             // up to N - 1 entries, one a lane
-#pragma unroll
-        for (uint32_t e = 0; e < N; e++) v[e] = -INFINITY;
-        if (lane < count) v[0] = to_f32(x[first + lane]);
-        pass.take(v, first + lane, lane < count ? 1 : 0);
-    };
+    Pass<T, TOP> pass;
+    // up to N - 1 entries, one a lane
+    auto few = [&](uint32_t first, uint32_t count) { pass.take(lane < count ? Vec<T>::one(x[first + lane]) : Vec<T>::nothing(), 0, false); };
     if (rank == 0 && warp == 0 && head) few(0, head);
     uint32_t i = v0 + tid;
     for (; i - tid + kThreads * kAhead <= v1; i += kThreads * kAhead) {
@@ -229,44 +296,79 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a, 
 #pragma unroll
         for (uint32_t j = 0; j < kAhead; j++) u[j] = __ldcs(xv + i + j * kThreads);
 #pragma unroll
-        for (uint32_t j = 0; j < kAhead; j++) {
-            Vec<T>::unpack(u[j], v);
-            pass.take(v, head + (i + j * kThreads) * N, N);
-        }
+        for (uint32_t j = 0; j < kAhead; j++) pass.take(u[j], i + j * kThreads, true);
     }
-    for (; i - lane < v1; i += kThreads) {
-        const bool in = i < v1;
-        if (in) Vec<T>::unpack(__ldcs(xv + i), v);
-        else {
+    {
+        uint4 u[kAhead];                       // what is left: all requested before the first is looked at
 #pragma unroll
-            for (uint32_t e = 0; e < N; e++) v[e] = -INFINITY;
-        }
-        pass.take(v, head + i * N, in ? N : 0);
+        for (uint32_t j = 0; j < kAhead; j++) u[j] = i + j * kThreads < v1 ? __ldcs(xv + i + j * kThreads) : Vec<T>::nothing();
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; j++)
+            if (i - lane + j * kThreads < v1) pass.take(u[j], i + j * kThreads, i + j * kThreads < v1);
     }
     if (rank == cluster - 1 && warp == kWarps - 1 && tail) few(head + vecs * N, tail);
     const Sums mine = pass.sums();
     if (lane == 0) part[warp] = mine;
-    if (TOP) tops[warp][lane] = pass.top;
-    __syncthreads();
     Top t = {0, 0};
+    if constexpr (TOP) {
+        // The k lanes with the largest entries have the k largest entries of all among theirs, whatever is larger than the k-th lane's: only those lanes' vectors
+        // are looked at again.  (Order by value, then by vector: of equal values in one vector all are taken.)
+        t = pass.top(v0 + tid, v1);
+        sort_lanes(t);
+        join_warps(t, lists);
+        const Top least = lists[0][a.k - 1];
+        Top found = {0, 0};
+        auto offer = [&](float y, uint32_t vec, uint32_t id, bool in) {      // entry `id` of a lane's vector `vec`
+            const uint32_t o = order(y);
+            uint32_t who = __ballot_sync(0xffffffffu, in && (o > least.v || (o == least.v && ~vec >= least.i)));
+            while (who) {
+                const uint32_t from = __ffs(who) - 1;
+                who &= who - 1;
+                insert(found, __shfl_sync(0xffffffffu, o, from), __shfl_sync(0xffffffffu, ~id, from));
+            }
+        };
+        uint32_t wide = 1;                     // threads of this warp that look at one lane's vectors: as many as it has, if that is fewer than 32
+        while (wide < 32 && wide * kThreads < v1 - v0) wide *= 2;
+        for (uint32_t q0 = warp * (32 / wide); q0 < a.k; q0 += kThreads / wide) {
+            const uint32_t q = q0 + lane / wide;
+            const Top s = q < a.k ? lists[0][q] : Top{0, 0};
+            const uint32_t first = s.v ? v0 + (~s.i - v0) % kThreads + lane % wide * kThreads : v1;
+            for (uint32_t j = 0; __any_sync(0xffffffffu, first + j < v1); j += kThreads * wide) {
+                const bool in = first + j < v1;
+                float v[N];
+                Vec<T>::unpack(in ? xv[first + j] : Vec<T>::nothing(), v);
+#pragma unroll
+                for (uint32_t e = 0; e < N; e++) offer(v[e], first + j, head + (first + j) * N + e, in);
+            }
+        }
+        // the entries outside of the vectors: those in front come before all others of their value, those behind after them
+        if (rank == 0 && warp == 0 && head) offer(lane < head ? to_f32(x[lane]) : 0.f, 0, lane, lane < head);
+        if (rank == cluster - 1 && warp == kWarps - 1 && tail) {
+            const uint32_t id = head + vecs * N + lane;
+            offer(lane < tail ? to_f32(x[id]) : 0.f, vecs, id, lane < tail);
+        }
+        __syncthreads();                       // `least` and the lanes have been read
+        t = found;
+        join_warps(t, lists);
+        if (warp == 0) best[lane] = t;
+    }
+    __syncthreads();
     if (warp == 0) {
         const Sums s = over_lanes(lane < kWarps ? part[lane] : Sums{-INFINITY, 0.f, 0.f});
         if (lane == 0) all = s;
-        if (TOP) {
-            t = pass.top;
-            for (uint32_t w = 1; w < kWarps; w++) join(t, tops[w][lane]);
-            best[lane] = t;
-        }
     }
     __syncwarp();
     if (cluster > 1) cluster_sync();
+    if (TOP && rank == 0 && cluster > 1) {     // a warp per block, or two
+        t = {0, 0};
+        for (uint32_t w = warp; w < cluster; w += kWarps)
+            join(t, Top{__float_as_uint(ld_cluster_f32(reinterpret_cast<const float*>(&best[lane].v), w)), __float_as_uint(ld_cluster_f32(reinterpret_cast<const float*>(&best[lane].i), w))});
+        join_warps(t, lists);
+    }
     if (rank == 0 && warp == 0) {
         Sums s{-INFINITY, 0.f, 0.f};
         if (lane < cluster) s = Sums{ld_cluster_f32(&all.m, lane), ld_cluster_f32(&all.z, lane), ld_cluster_f32(&all.b, lane)};
         s = over_lanes(s);
-        if (TOP)
-            for (uint32_t w = 1; w < cluster; w++)
-                join(t, Top{__float_as_uint(ld_cluster_f32(reinterpret_cast<const float*>(&best[lane].v), w)), __float_as_uint(ld_cluster_f32(reinterpret_cast<const float*>(&best[lane].i), w))});
         const bool none = s.m == -INFINITY;
         if (s.m == INFINITY) s.z = NAN;        // Inf - Inf, as the formula has it
         const float logz = log1pf(s.z);
