@@ -4,6 +4,7 @@
 // and log Z = log1p(z): when that entry holds nearly all of the mass, its log probability and the entropy are tiny and keep their digits.
 #include "gemv_common.cuh"
 #include "paged.cuh"
+#include "tcgen05.cuh"
 #include "tma.cuh"
 
 namespace runit {
@@ -16,11 +17,13 @@ struct Args {
     const int32_t* tokens;
     float *logprob, *entropy, *top_logprobs;
     int32_t* top_ids;
-    uint32_t ld, n, k;
+    int32_t* status;
+    uint32_t ld, n, k, rows;
 };
 
-constexpr uint32_t kThreads = 256, kWarps = kThreads / 32;
-constexpr float kLog2e = 1.4426950408889634f, kLeast = -200.f;      // e^-200 is 0 in f32
+constexpr uint32_t kThreads = 256, kWarps = kThreads / 32 - 1, kAhead = 4, kStages = 3;     // kWarps read; one more adds up what they have found
+constexpr uint32_t kStageVecs = 32 * kAhead, kStageBytes = 16 * kStageVecs, kBlocksPerSm = 4;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kLeast = -200.f;      // e^-200 is 0 in f32
 
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
@@ -86,13 +89,13 @@ __device__ __forceinline__ void join(Top& t, const Top& o) {
     }
 }
 
-constexpr float kFloor = -1e38f;               // -Inf in the fast path, where the maximum is above kLow, so far above that the floor has no mass
+constexpr float kFloor = -1e38f;               // -Inf in the fast path, where the maximum is within kFar: far above the floor, and R is rounded by less than 2^-7
 
 // Sixteen bytes of logits: unpacked; their maximum (a NaN stays one); unpacked with -Inf raised to the floor (f16: to its lowest number).
 template <typename T> struct Vec;
 template <> struct Vec<float> {
     static constexpr uint32_t N = 4;
-    static constexpr float kLow = -1e37f;
+    static constexpr float kFar = 1e5f;
     static __device__ __forceinline__ void unpack(const uint4& u, float (&v)[4]) {
         v[0] = __uint_as_float(u.x); v[1] = __uint_as_float(u.y); v[2] = __uint_as_float(u.z); v[3] = __uint_as_float(u.w);
     }
@@ -105,11 +108,18 @@ template <> struct Vec<float> {
         for (int i = 0; i < 4; i++) v[i] = fmaxf(v[i], kFloor);
     }
     static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u); }
+    // the first entry that is m becomes -Inf
+    static __device__ __forceinline__ void drop(uint4& u, float m, bool& leave) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (leave && __uint_as_float(w[i]) == m) { w[i] = 0xFF800000u; leave = false; }
+    }
     static __device__ __forceinline__ uint4 one(float v) { return make_uint4(__float_as_uint(v), 0xFF800000u, 0xFF800000u, 0xFF800000u); }
 };
 template <> struct Vec<__half> {
     static constexpr uint32_t N = 8;
-    static constexpr float kLow = -6e4f;
+    static constexpr float kFar = 6e4f;
     static __device__ __forceinline__ void unpack(const uint4& u, float (&v)[8]) {
         const __half2* h = reinterpret_cast<const __half2*>(&u);
 #pragma unroll
@@ -132,11 +142,22 @@ template <> struct Vec<__half> {
         unpack(r, v);
     }
     static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u); }
+    static __device__ __forceinline__ void drop(uint4& u, float m, bool& leave) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int q = 0; q < 2; q++)
+                if (leave && __half2float(__ushort_as_half((unsigned short)(w[i] >> 16 * q))) == m) {
+                    w[i] = (w[i] & (0xFFFF0000u >> 16 * q)) | (0xFC00u << 16 * q);
+                    leave = false;
+                }
+    }
     static __device__ __forceinline__ uint4 one(__half v) { return make_uint4(0xFC000000u | __half_as_ushort(v), 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u); }
 };
 template <> struct Vec<__nv_bfloat16> {
     static constexpr uint32_t N = 8;
-    static constexpr float kLow = -1e37f;
+    static constexpr float kFar = 1e5f;
     static __device__ __forceinline__ void unpack(const uint4& u, float (&v)[8]) {
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -158,56 +179,110 @@ template <> struct Vec<__nv_bfloat16> {
         unpack(r, v);
     }
     static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u); }
+    static __device__ __forceinline__ void drop(uint4& u, float m, bool& leave) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int q = 0; q < 2; q++)
+                if (leave && __uint_as_float((w[i] >> 16 * q) << 16) == m) {
+                    w[i] = (w[i] & (0xFFFF0000u >> 16 * q)) | (0xFF80u << 16 * q);
+                    leave = false;
+                }
+    }
     static __device__ __forceinline__ uint4 one(__nv_bfloat16 v) { return make_uint4(0xFF800000u | __bfloat16_as_ushort(v), 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u); }
 };
 
-// A warp's pass over its share of a row, in the order of the indices.  The maximum is the warp's: it rises some ten times in a share, and only
-// then are the sums scaled; one lane leaves the maximal entry out.
+// A warp's pass over its share of a row, in the order of the indices.  The maximum is the warp's: it rises some five to ten times in a share, and only
+// then are the sums scaled; one lane leaves the maximal entry out.  Below the maximum an entry is one multiply-add, t = x log2 e - R with R = m log2 e
+// rounded, 2^t and the sums of 2^t and 2^t t; what R was rounded by (e) goes into the sums when they are handed over.
 template <typename T, bool TOP> struct Pass {
     static constexpr uint32_t N = Vec<T>::N;
-    float m = -INFINITY, mine = -INFINITY;     // of the warp; of the lane's vectors
-    uint32_t owner = 32, at = 0xFFFFFFFFu;     // the lane that has left an entry out; the lane's first vector that has `mine`
-    uint64_t z2 = 0, b2 = 0;
+    float m = -INFINITY;
+    uint32_t owner = 32;                       // the lane that has left an entry out
+    float mine = -INFINITY, second = -INFINITY;                  // the largest entries of the lane's vectors: of one, and of the others
+    uint32_t at = 0xFFFFFFFFu;                 // the first vector that has `mine`
+    bool nan = false, leave = false;
+    float z = 0.f, b = 0.f, r = 0.f;           // sums of e^d and e^d d relative to m; R
+    uint64_t z2 = 0, b2 = 0;                   // sums of 2^t and 2^t t since m has risen
 
-    // vector i of the row (-Inf where there is nothing; `in`: it counts among the lane's)
-    __device__ __forceinline__ void take(const uint4& u, uint32_t i, bool in) {
-        const float most = Vec<T>::most(u);
-        const bool up = !(most <= m);
-        if (__any_sync(0xffffffffu, up || m < Vec<T>::kLow)) {
-            rise(u, most, i, in);
-            return;
+    __device__ __forceinline__ void hand_over() {
+        const float e = fmaf(m, kLog2e, -r), f = exp2_approx(-e), zt = sum2(z2), bt = sum2(b2);
+        if (zt != 0.f) {                       // else nothing was added (and m need not be a number)
+            z = fmaf(f, zt, z);
+            b = fmaf(f * kLn2, fmaf(-e, zt, bt), b);
         }
-        if (TOP && most > mine && in) { mine = most; at = i; }
-        float v[N];
-        Vec<T>::raised(u, v);
-        const uint64_t sub2 = packf(-m), l2 = packf(kLog2e);
+        z2 = b2 = 0;
+    }
+    // vectors i, i + 32, ... of the row, -Inf where there is nothing
+    template <int V> __device__ __forceinline__ void take(uint4 (&u)[V], uint32_t i) {
+        float most[V], all = -INFINITY;
 #pragma unroll
-        for (uint32_t e = 0; e < N; e += 2) {
-            const uint64_t d = fadd2(pack2(__float_as_uint(v[e]), __float_as_uint(v[e + 1])), sub2), t = fmul2(d, l2);
-            const uint64_t p = pack2(__float_as_uint(exp2_approx(__uint_as_float((uint32_t)t))), __float_as_uint(exp2_approx(__uint_as_float((uint32_t)(t >> 32)))));
-            z2 = fadd2(z2, p);
-            b2 = ffma2(p, d, b2);
+        for (int j = 0; j < V; j++) {
+            most[j] = Vec<T>::most(u[j]);
+            all = max_nan(all, most[j]);
+        }
+        if (__any_sync(0xffffffffu, !(all <= m) || !(fabsf(m) < Vec<T>::kFar))) {
+            if (!rise(all)) {                  // no number, or far out
+#pragma unroll
+                for (int j = 0; j < V; j++) plain(u[j], most[j], i + 32 * j);
+                return;
+            }
+            if (leave) {                       // the entry goes where the floor is; it has been noted with its vector
+#pragma unroll
+                for (int j = 0; j < V; j++)
+                    if (leave && most[j] == m) Vec<T>::drop(u[j], m, leave);
+            }
+        }
+        const uint64_t r2 = packf(-r), l2 = packf(kLog2e);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            if (TOP) note(most[j], i + 32 * j);
+            float v[N];
+            Vec<T>::raised(u[j], v);
+#pragma unroll
+            for (uint32_t e = 0; e < N; e += 2) {
+                const uint64_t t = ffma2(pack2(__float_as_uint(v[e]), __float_as_uint(v[e + 1])), l2, r2);
+                const uint64_t p = pack2(__float_as_uint(exp2_approx(__uint_as_float((uint32_t)t))), __float_as_uint(exp2_approx(__uint_as_float((uint32_t)(t >> 32)))));
+                z2 = fadd2(z2, p);
+                b2 = ffma2(p, t, b2);
+            }
         }
     }
-    // the same where the maximum rises, is no number or is very low
-    __device__ __forceinline__ void rise(const uint4& u, float most, uint32_t i, bool in) {
+    __device__ __forceinline__ void note(float most, uint32_t i) {
+        second = fmaxf(second, fminf(mine, most));
+        if (most > mine) { mine = most; at = i; }
+    }
+    // The warp's maximum becomes that of `all` too, if that is larger: the sums are scaled, one lane has an entry to leave out.  Whether 2^t can follow.
+    __device__ __forceinline__ bool rise(float all) {
         const uint32_t lane = threadIdx.x & 31;
-        if (TOP && in && (most > mine || (most != most && mine == mine))) { mine = most; at = i; }
-        bool leave = false;
-        if (__any_sync(0xffffffffu, !(most <= m))) {
-            float now = max_nan(m, most);
+        leave = false;
+        if (__any_sync(0xffffffffu, !(all <= m))) {
+            float now = max_nan(m, all);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) now = max_nan(now, __shfl_xor_sync(0xffffffffu, now, o));
+            hand_over();
             const float d = m == -INFINITY ? kLeast : m - now, w = m == -INFINITY ? 0.f : exp_of(d);
-            const float z = sum2(z2) + (lane == owner ? 1.f : 0.f), b = sum2(b2);         // with what was left out so far
-            z2 = pack2(__float_as_uint(w * z), 0);
-            b2 = pack2(__float_as_uint(w * fmaf(d, z, b)), 0);
+            if (lane == owner) z += 1.f;       // what was left out so far
+            b = w * fmaf(d, z, b);
+            z *= w;
             m = now;
-            owner = __ffs(__ballot_sync(0xffffffffu, most == now)) - 1;
+            r = m * kLog2e;
+            owner = __ffs(__ballot_sync(0xffffffffu, all == now)) - 1;
             leave = lane == owner;
         }
+        return fabsf(m) < Vec<T>::kFar;
+    }
+    // a vector by its differences from the maximum
+    __device__ __forceinline__ void plain(const uint4& u, float most, uint32_t i) {
+        if (TOP) {
+            if (most != most) {
+                if (!nan) { mine = most; at = i; }
+                nan = true;
+            } else if (!nan) note(most, i);
+        }
         const float sub = m == -INFINITY ? 0.f : m;
-        float v[N], z = 0.f, b = 0.f;
+        float v[N];
         Vec<T>::unpack(u, v);
 #pragma unroll
         for (uint32_t e = 0; e < N; e++) {
@@ -217,42 +292,25 @@ template <typename T, bool TOP> struct Pass {
             z += p;
             b = fmaf(p, d, b);
         }
-        z2 = fadd2(z2, pack2(__float_as_uint(z), 0));
-        b2 = fadd2(b2, pack2(__float_as_uint(b), 0));
     }
     // the lane's largest entry; first: its first vector, if it has any
     __device__ __forceinline__ Top top(uint32_t first, uint32_t end) const {
         if (at != 0xFFFFFFFFu) return Top{order(mine), ~at};
         return first < end ? Top{order(-INFINITY), ~first} : Top{0, 0};
     }
-    __device__ __forceinline__ Sums sums() const {
-        Sums s{m, sum2(z2), sum2(b2)};
-        float z = s.z, b = s.b;
+    // what the lane's other vectors have at most
+    __device__ __forceinline__ uint32_t others() const { return nan ? 0xFFFFFFFFu : order(second); }
+    __device__ __forceinline__ Sums sums() {
+        hand_over();
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             z += __shfl_xor_sync(0xffffffffu, z, o);
             b += __shfl_xor_sync(0xffffffffu, b, o);
         }
-        s.z = z;
-        s.b = b;
-        return s;
+        return Sums{m, z, b};
     }
 };
 
-// The lists of a block's warps joined: the result in warp 0.  All threads.
-__device__ __forceinline__ void join_warps(Top& t, Top (*lists)[32]) {
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    lists[warp][lane] = t;
-    __syncthreads();
-#pragma unroll
-    for (uint32_t w = kWarps / 2; w > 0; w /= 2) {
-        if (warp < w) {
-            join(t, lists[warp + w][lane]);
-            lists[warp][lane] = t;
-        }
-        __syncthreads();
-    }
-}
 // Descending order of the lanes' entries.
 __device__ __forceinline__ void sort_lanes(Top& t) {
     const uint32_t lane = threadIdx.x & 31;
@@ -266,124 +324,227 @@ __device__ __forceinline__ void sort_lanes(Top& t) {
         }
 }
 
-// A cluster of `cluster` blocks per row (a power of two up to 16), each with a run of the row; the first one adds up.
+// Counted on mbarriers, with the suspension of mbar_try: a warp that polls takes issue slots from those that have data.
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
+    for (uint32_t i = 0; i < kSpinLimit; i++)
+        if (mbar_try(bar, parity)) return true;
+    return false;
+}
+
+// A block takes rows blockIdx.x / cluster, + gridDim.x, ...; with few rows a cluster of `cluster` blocks (a power of two up to 16) shares one, and the first of them
+// adds up.  Seven warps read: each has a run of the row's 16-byte vectors, which come by bulk copies of 2 KB into its own ring of three, and goes on to its
+// run of the next row; the eighth warp turns what they have found into the row's results, one row behind.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a, const uint32_t cluster) {
-    constexpr uint32_t N = Vec<T>::N, kAhead = 4;
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(const Args a, const uint32_t cluster) {
+    constexpr uint32_t N = Vec<T>::N;
+    extern __shared__ __align__(128) uint8_t ring[];             // [kWarps][kStages][kStageBytes]
+    __shared__ __align__(8) uint64_t bars[kWarps * kStages + 4];
+    __shared__ Sums part[2][kWarps], all;
+    __shared__ Top lists[2][kWarps][32], best[32];
+    __shared__ uint32_t seconds[2][kWarps][32];
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, rank = blockIdx.x % cluster;
+    if (tid < kWarps * kStages + 4) mbar_init(smem_u32(&bars[tid]), tid >= kWarps * kStages && tid < kWarps * kStages + 2 ? kWarps : 1);
+    fence_mbar_init();
+    __syncthreads();
     grid_dependency_wait();
     grid_launch_dependents();
-    __shared__ Sums part[kWarps], all;
-    __shared__ Top lists[kWarps][32], best[32];
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.x / cluster, rank = blockIdx.x % cluster;
-    const T* x = reinterpret_cast<const T*>(a.x) + (size_t)row * a.ld;
-    // entries ahead of the first 16-byte boundary, whole vectors, entries behind the last
-    const uint32_t head = min(a.n, (uint32_t)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T))), vecs = (a.n - head) / N, tail = a.n - head - vecs * N;
-    const uint32_t per = (vecs + cluster - 1) / cluster, v0 = min(vecs, rank * per), v1 = min(vecs, v0 + per);
-    const uint4* const xv = reinterpret_cast<const uint4*>(x + head);
-    int32_t token = 0;
-    float xt = 0.f;
-    if (rank == 0 && tid == 0 && a.tokens) {
-        token = a.tokens[row];
-        if ((uint32_t)token < a.n) xt = to_f32(x[token]);
-    }
-    Pass<T, TOP> pass;
-    // up to N - 1 entries, one a lane
-    auto few = [&](uint32_t first, uint32_t count) { pass.take(lane < count ? Vec<T>::one(x[first + lane]) : Vec<T>::nothing(), 0, false); };
-    if (rank == 0 && warp == 0 && head) few(0, head);
-    uint32_t i = v0 + tid;
-    for (; i - tid + kThreads * kAhead <= v1; i += kThreads * kAhead) {
-        uint4 u[kAhead];
-#pragma unroll
-        for (uint32_t j = 0; j < kAhead; j++) u[j] = __ldcs(xv + i + j * kThreads);
-#pragma unroll
-        for (uint32_t j = 0; j < kAhead; j++) pass.take(u[j], i + j * kThreads, true);
-    }
-    {
-        uint4 u[kAhead];                       // what is left: all requested before the first is looked at
-#pragma unroll
-        for (uint32_t j = 0; j < kAhead; j++) u[j] = i + j * kThreads < v1 ? __ldcs(xv + i + j * kThreads) : Vec<T>::nothing();
-#pragma unroll
-        for (uint32_t j = 0; j < kAhead; j++)
-            if (i - lane + j * kThreads < v1) pass.take(u[j], i + j * kThreads, i + j * kThreads < v1);
-    }
-    if (rank == cluster - 1 && warp == kWarps - 1 && tail) few(head + vecs * N, tail);
-    const Sums mine = pass.sums();
-    if (lane == 0) part[warp] = mine;
+    const uint32_t there = smem_u32(&bars[kWarps * kStages]), taken = there + 16;          // of the two buffers that hold a row's findings
+    // A row: entries ahead of the first 16-byte boundary, whole vectors, entries behind the last; the block's vectors v0 .. v1 - 1, a warp's `share`.
+    struct Run {
+        const T* x;
+        uint32_t head, vecs, tail, v0, v1, share;
+    };
+    auto run_of = [&](uint32_t row) {
+        Run r;
+        r.x = reinterpret_cast<const T*>(a.x) + (size_t)row * a.ld;
+        r.head = min(a.n, (uint32_t)((16 - (reinterpret_cast<uintptr_t>(r.x) & 15)) % 16 / sizeof(T)));
+        r.vecs = (a.n - r.head) / N;
+        r.tail = a.n - r.head - r.vecs * N;
+        const uint32_t per = (r.vecs + cluster - 1) / cluster;
+        r.v0 = min(r.vecs, rank * per);
+        r.v1 = min(r.vecs, r.v0 + per);
+        r.share = ((r.v1 - r.v0 + kWarps - 1) / kWarps + 31) / 32 * 32;
+        return r;
+    };
+    bool ok = true;
+    Sums s{-INFINITY, 0.f, 0.f};               // of the warp that adds up: the block's, in the end
     Top t = {0, 0};
-    if constexpr (TOP) {
-        // The k lanes with the largest entries have the k largest entries of all among theirs, whatever is larger than the k-th lane's: only those lanes' vectors
-        // are looked at again.  (Order by value, then by vector: of equal values in one vector all are taken.)
-        t = pass.top(v0 + tid, v1);
-        sort_lanes(t);
-        join_warps(t, lists);
-        const Top least = lists[0][a.k - 1];
-        Top found = {0, 0};
-        auto offer = [&](float y, uint32_t vec, uint32_t id, bool in) {      // entry `id` of a lane's vector `vec`
-            const uint32_t o = order(y);
-            uint32_t who = __ballot_sync(0xffffffffu, in && (o > least.v || (o == least.v && ~vec >= least.i)));
-            while (who) {
-                const uint32_t from = __ffs(who) - 1;
-                who &= who - 1;
-                insert(found, __shfl_sync(0xffffffffu, o, from), __shfl_sync(0xffffffffu, ~id, from));
+    uint32_t turn = 0;
+    if (warp < kWarps) {
+        const uint4* const mine = reinterpret_cast<const uint4*>(ring + warp * kStages * kStageBytes);
+        const uint32_t mine_s = smem_u32(mine), bar0 = smem_u32(&bars[warp * kStages]);
+        uint32_t asked = 0, used = 0;          // copies of this warp so far
+        // the run's copies that have been asked for go on into the next row's
+        uint32_t ask_row = blockIdx.x / cluster, ask_at = 0;
+        Run q = run_of(ask_row);
+        auto ask = [&]() {
+            while (ask_row < a.rows) {
+                const uint32_t w0 = min(q.v1, q.v0 + warp * q.share), w1 = min(q.v1, w0 + q.share), v = w0 + ask_at;
+                if (v < w1) {
+                    if (lane == 0) {
+                        const uint32_t slot = asked % kStages, bar = bar0 + 8 * slot, bytes = 16 * min(kStageVecs, w1 - v);
+                        mbar_expect_tx(bar, bytes);
+                        bulk_load_1d(mine_s + slot * kStageBytes, reinterpret_cast<const uint4*>(q.x + q.head) + v, bytes, bar);
+                    }
+                    asked++;
+                    ask_at += kStageVecs;
+                    return;
+                }
+                ask_row += cluster > 1 ? a.rows : gridDim.x;
+                ask_at = 0;
+                if (ask_row < a.rows) q = run_of(ask_row);
             }
         };
-        uint32_t wide = 1;                     // threads of this warp that look at one lane's vectors: as many as it has, if that is fewer than 32
-        while (wide < 32 && wide * kThreads < v1 - v0) wide *= 2;
-        for (uint32_t q0 = warp * (32 / wide); q0 < a.k; q0 += kThreads / wide) {
-            const uint32_t q = q0 + lane / wide;
-            const Top s = q < a.k ? lists[0][q] : Top{0, 0};
-            const uint32_t first = s.v ? v0 + (~s.i - v0) % kThreads + lane % wide * kThreads : v1;
-            for (uint32_t j = 0; __any_sync(0xffffffffu, first + j < v1); j += kThreads * wide) {
-                const bool in = first + j < v1;
-                float v[N];
-                Vec<T>::unpack(in ? xv[first + j] : Vec<T>::nothing(), v);
+        for (uint32_t i = 0; i < kStages; i++) ask();
+        for (uint32_t row = blockIdx.x / cluster; row < a.rows; row += cluster > 1 ? a.rows : gridDim.x, turn++) {
+            const Run r = run_of(row);
+            const uint32_t w0 = min(r.v1, r.v0 + warp * r.share), w1 = min(r.v1, w0 + r.share), half = turn & 1;
+            Pass<T, TOP> pass;
+            // up to N - 1 entries, one a lane
+            auto few = [&](uint32_t first, uint32_t count) {
+                const uint4 u = lane < count ? Vec<T>::one(r.x[first + lane]) : Vec<T>::nothing();
+                const auto was = pass;         // they do not count among the lane's vectors
+                pass.rise(Vec<T>::most(u));
+                pass.plain(u, Vec<T>::most(u), 0);
+                pass.mine = was.mine; pass.second = was.second; pass.at = was.at; pass.nan = was.nan;
+            };
+            if (rank == 0 && warp == 0 && r.head) few(0, r.head);
+            for (uint32_t v = w0; v < w1; v += kStageVecs) {
+                const uint32_t slot = used % kStages;
+                const uint4* const from = mine + slot * kStageVecs + lane;
+                if (ok) ok = __all_sync(0xffffffffu, wait(bar0 + 8 * slot, (used / kStages) & 1));
+                uint4 u[kAhead];
+                if (v + kStageVecs <= w1) {
 #pragma unroll
-                for (uint32_t e = 0; e < N; e++) offer(v[e], first + j, head + (first + j) * N + e, in);
+                    for (uint32_t j = 0; j < kAhead; j++) u[j] = from[32 * j];
+                } else {
+#pragma unroll
+                    for (uint32_t j = 0; j < kAhead; j++) u[j] = v + 32 * j + lane < w1 ? from[32 * j] : Vec<T>::nothing();
+                }
+                used++;
+                __syncwarp();
+                if (ok) ask();
+                pass.take(u, v + lane);
             }
+            if (rank == cluster - 1 && warp == kWarps - 1 && r.tail) few(r.head + r.vecs * N, r.tail);
+            const Sums sums = pass.sums();
+            if (turn >= 2 && ok) ok = __all_sync(0xffffffffu, wait(taken + 8 * half, (turn / 2 - 1) & 1));
+            if (lane == 0) part[half][warp] = sums;
+            if constexpr (TOP) {
+                seconds[half][warp][lane] = pass.others();
+                Top top = pass.top(w0 + lane, w1);
+                sort_lanes(top);
+                lists[half][warp][lane] = top;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(there + 8 * half);
         }
-        // the entries outside of the vectors: those in front come before all others of their value, those behind after them
-        if (rank == 0 && warp == 0 && head) offer(lane < head ? to_f32(x[lane]) : 0.f, 0, lane, lane < head);
-        if (rank == cluster - 1 && warp == kWarps - 1 && tail) {
-            const uint32_t id = head + vecs * N + lane;
-            offer(lane < tail ? to_f32(x[id]) : 0.f, vecs, id, lane < tail);
-        }
-        __syncthreads();                       // `least` and the lanes have been read
-        t = found;
-        join_warps(t, lists);
-        if (warp == 0) best[lane] = t;
+        if (!ok) mbar_drain(bar0, kStages, asked);               // nothing is in flight when the block leaves
     }
-    __syncthreads();
-    if (warp == 0) {
-        const Sums s = over_lanes(lane < kWarps ? part[lane] : Sums{-INFINITY, 0.f, 0.f});
-        if (lane == 0) all = s;
-    }
-    __syncwarp();
-    if (cluster > 1) cluster_sync();
-    if (TOP && rank == 0 && cluster > 1) {     // a warp per block, or two
-        t = {0, 0};
-        for (uint32_t w = warp; w < cluster; w += kWarps)
-            join(t, Top{__float_as_uint(ld_cluster_f32(reinterpret_cast<const float*>(&best[lane].v), w)), __float_as_uint(ld_cluster_f32(reinterpret_cast<const float*>(&best[lane].i), w))});
-        join_warps(t, lists);
-    }
-    if (rank == 0 && warp == 0) {
-        Sums s{-INFINITY, 0.f, 0.f};
-        if (lane < cluster) s = Sums{ld_cluster_f32(&all.m, lane), ld_cluster_f32(&all.z, lane), ld_cluster_f32(&all.b, lane)};
-        s = over_lanes(s);
+    auto result = [&](uint32_t row) {          // of a row whose sums and alternatives are in s and t
+        const T* const x = reinterpret_cast<const T*>(a.x) + (size_t)row * a.ld;
         const bool none = s.m == -INFINITY;
         if (s.m == INFINITY) s.z = NAN;        // Inf - Inf, as the formula has it
         const float logz = log1pf(s.z);
         auto log_of = [&](float y) { return y == -INFINITY && s.m == s.m && s.z == s.z ? -INFINITY : y - s.m - logz; };
         if (lane == 0) {
             if (a.entropy) a.entropy[row] = none ? 0.f : s.m == s.m ? logz - s.b / (1.f + s.z) : NAN;
-            if (a.tokens) a.logprob[row] = (uint32_t)token < a.n ? log_of(xt) : 0.f;
+            if (a.tokens) {
+                const int32_t token = a.tokens[row];
+                a.logprob[row] = (uint32_t)token < a.n ? log_of(to_f32(x[token])) : 0.f;
+            }
         }
         if (TOP && lane < a.k) {
             a.top_ids[(size_t)row * a.k + lane] = (int32_t)~t.i;
             a.top_logprobs[(size_t)row * a.k + lane] = log_of(value(t.v));
         }
+    };
+    if (warp == kWarps) {
+        for (uint32_t row = blockIdx.x / cluster; row < a.rows; row += cluster > 1 ? a.rows : gridDim.x, turn++) {
+            const Run r = run_of(row);
+            const uint32_t half = turn & 1;
+            if (ok) ok = __all_sync(0xffffffffu, wait(there + 8 * half, (turn / 2) & 1));
+            s = over_lanes(lane < kWarps ? part[half][lane] : Sums{-INFINITY, 0.f, 0.f});
+            if constexpr (TOP) {
+                // The k lanes (of the block) with the largest entries have the k largest entries among theirs, whatever is larger than the k-th lane's: in the
+                // vector that holds the lane's largest, and where its others reach as high, in all of them.  (Order by value, then by vector: of equal
+                // values in one vector all are taken.)
+                t = lists[half][0][lane];
+                for (uint32_t w = 1; w < kWarps; w++) join(t, lists[half][w][lane]);
+                const Top least = {__shfl_sync(0xffffffffu, t.v, a.k - 1), __shfl_sync(0xffffffffu, t.i, a.k - 1)};
+                const uint4* const xv = reinterpret_cast<const uint4*>(r.x + r.head);
+                Top found = {0, 0};
+                auto offer = [&](float y, uint32_t vec, uint32_t id, bool in) {    // entry `id` of a lane's vector `vec`
+                    const uint32_t o = order(y);
+                    uint32_t who = __ballot_sync(0xffffffffu, in && (o > least.v || (o == least.v && ~vec >= least.i)));
+                    while (who) {
+                        const uint32_t from = __ffs(who) - 1;
+                        who &= who - 1;
+                        insert(found, __shfl_sync(0xffffffffu, o, from), __shfl_sync(0xffffffffu, ~id, from));
+                    }
+                };
+                auto offer_vector = [&](uint32_t vec, bool in) {
+                    const uint4 u = in ? xv[vec] : Vec<T>::nothing();
+                    float v[N];
+                    Vec<T>::unpack(u, v);
+#pragma unroll
+                    for (uint32_t e = 0; e < N; e++) offer(v[e], vec, r.head + vec * N + e, in);
+                };
+                const bool mine = lane < a.k && t.v;
+                const uint32_t vec = ~t.i, run = mine ? (vec - r.v0) / r.share : 0, run0 = r.v0 + run * r.share, first = run0 + (vec - run0) % 32;
+                const bool whole = mine && ok && seconds[half][run][first - run0] >= least.v;
+                offer_vector(vec, mine && ok && !whole);
+                uint32_t again = __ballot_sync(0xffffffffu, whole);
+                while (again) {
+                    const uint32_t from = __ffs(again) - 1, f = __shfl_sync(0xffffffffu, first, from), end = min(r.v1, __shfl_sync(0xffffffffu, run0, from) + r.share);
+                    again &= again - 1;
+                    for (uint32_t j = f; j < end; j += 32 * 32) offer_vector(j + 32 * lane, j + 32 * lane < end);
+                }
+                // the entries outside of the vectors: those in front come before all others of their value, those behind after them
+                if (rank == 0 && r.head) offer(lane < r.head ? to_f32(r.x[lane]) : 0.f, 0, lane, lane < r.head);
+                if (rank == cluster - 1 && r.tail) {
+                    const uint32_t id = r.head + r.vecs * N + lane;
+                    offer(lane < r.tail ? to_f32(r.x[id]) : 0.f, r.vecs, id, lane < r.tail);
+                }
+                t = found;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(taken + 8 * half);
+            if (cluster == 1) result(row);
+        }
+        if (cluster > 1) {
+            if (lane == 0) all = s;
+            best[lane] = t;
+        }
     }
-    __syncwarp();
-    if (cluster > 1) cluster_sync();           // the others' sums are read by then
+    if (!ok && lane == 0 && a.status) atomicCAS(a.status, 0, 1);
+    if (cluster > 1) {                         // the blocks' results meet in the first one
+        __syncwarp();
+        cluster_sync();
+        if (rank == 0) {
+            if (TOP) {                         // a warp has two or three blocks' lists, then one warp the warps'
+                if (warp < kWarps) {
+                    t = {0, 0};
+                    for (uint32_t w = warp; w < cluster; w += kWarps)
+                        join(t, Top{__float_as_uint(ld_cluster_f32(reinterpret_cast<const float*>(&best[lane].v), w)), __float_as_uint(ld_cluster_f32(reinterpret_cast<const float*>(&best[lane].i), w))});
+                    lists[0][warp][lane] = t;
+                }
+                __syncthreads();
+                if (warp == kWarps) {
+                    t = lists[0][0][lane];
+                    for (uint32_t w = 1; w < kWarps; w++) join(t, lists[0][w][lane]);
+                }
+            }
+            if (warp == kWarps) {
+                s = Sums{-INFINITY, 0.f, 0.f};
+                if (lane < cluster) s = Sums{ld_cluster_f32(&all.m, lane), ld_cluster_f32(&all.z, lane), ld_cluster_f32(&all.b, lane)};
+                s = over_lanes(s);
+                result(blockIdx.x / cluster);
+            }
+        }
+        __syncwarp();
+        cluster_sync();                        // the others' shared memory is read by then
+    }
 }
 
 // Blocks of a row: enough rows fill the GPU by themselves; a block has 2048 entries at least.
@@ -392,15 +553,18 @@ static uint32_t cluster_of(uint32_t rows, uint32_t n) {
     while (c < 16 && (uint64_t)rows * c * 2 <= 2 * 148 && n / (c * 2) >= 2048) c *= 2;
     return c;
 }
-template <typename T, bool TOP> static int32_t run(runit_ctx* ctx, const Args& a, uint32_t rows) {
-    const uint32_t cluster = cluster_of(rows, a.n);
+template <typename T, bool TOP> static int32_t run(runit_ctx* ctx, const Args& a) {
+    constexpr uint32_t smem = kWarps * kStages * kStageBytes;
+    const uint32_t cluster = cluster_of(a.rows, a.n);
     static bool configured[64] = {false};
     if (ctx->device >= 64 || !configured[ctx->device]) {
         RUNIT_CUDA_TRY(ctx, cudaFuncSetAttribute(token_logprobs_kernel<T, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        RUNIT_CUDA_TRY(ctx, cudaFuncSetAttribute(token_logprobs_kernel<T, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         if (ctx->device < 64) configured[ctx->device] = true;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(rows * cluster);
+    cfg.gridDim = dim3(cluster > 1 ? a.rows * cluster : min(a.rows, (uint32_t)ctx->sm_count * kBlocksPerSm));
+    cfg.dynamicSmemBytes = smem;
     cfg.blockDim = dim3(kThreads);
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[2];
@@ -424,15 +588,15 @@ extern "C" int32_t runit_token_logprobs(runit_ctx_t* ctx, const void* logits, in
                                         void* logprob, void* entropy, uint32_t k, void* top_ids, void* top_logprobs) {
     if (!ctx) return RUNIT_ERR_BAD_ARG;
     RUNIT_REQUIRE(ctx, type >= RUNIT_TYPE_F32 && type <= RUNIT_TYPE_BF16, "token_logprobs: type %d", type);
-    RUNIT_REQUIRE(ctx, logits && n > 0 && rows > 0 && ld >= n && n <= 0x7FFFFFFFu && rows <= 0x7FFFFFFFu / 16, "token_logprobs: null logits, n=%u, rows=%u or ld=%u", n, rows, ld);
+    RUNIT_REQUIRE(ctx, logits && n > 0 && rows > 0 && ld >= n && n <= 0x7FFFFFFFu && rows <= 0x7FFFFFFFu, "token_logprobs: null logits, n=%u, rows=%u or ld=%u", n, rows, ld);
     RUNIT_REQUIRE(ctx, runit_aligned(logits, type == RUNIT_TYPE_F32 ? 4 : 2), "token_logprobs: misaligned logits");
     RUNIT_REQUIRE(ctx, (tokens != nullptr) == (logprob != nullptr), "token_logprobs: tokens and logprob come together");
     RUNIT_REQUIRE(ctx, k <= 32 && k <= n && (k > 0) == (top_ids != nullptr) && (k > 0) == (top_logprobs != nullptr), "token_logprobs: k=%u must be at most 32 and n, with top_ids and top_logprobs", k);
     RUNIT_REQUIRE(ctx, logprob || entropy || k > 0, "token_logprobs: nothing is asked for");
     RUNIT_REQUIRE(ctx, runit_aligned(tokens, 4) && runit_aligned(logprob, 4) && runit_aligned(entropy, 4) && runit_aligned(top_ids, 4) && runit_aligned(top_logprobs, 4),
                   "token_logprobs: misaligned tokens or results");
-    const lp::Args a{logits, (const int32_t*)tokens, (float*)logprob, (float*)entropy, (float*)top_logprobs, (int32_t*)top_ids, ld, n, k};
-    if (type == RUNIT_TYPE_F32) return k ? lp::run<float, true>(ctx, a, rows) : lp::run<float, false>(ctx, a, rows);
-    if (type == RUNIT_TYPE_F16) return k ? lp::run<__half, true>(ctx, a, rows) : lp::run<__half, false>(ctx, a, rows);
-    return k ? lp::run<__nv_bfloat16, true>(ctx, a, rows) : lp::run<__nv_bfloat16, false>(ctx, a, rows);
+    const lp::Args a{logits, (const int32_t*)tokens, (float*)logprob, (float*)entropy, (float*)top_logprobs, (int32_t*)top_ids, ctx->d_status, ld, n, k, rows};
+    if (type == RUNIT_TYPE_F32) return k ? lp::run<float, true>(ctx, a) : lp::run<float, false>(ctx, a);
+    if (type == RUNIT_TYPE_F16) return k ? lp::run<__half, true>(ctx, a) : lp::run<__half, false>(ctx, a);
+    return k ? lp::run<__nv_bfloat16, true>(ctx, a) : lp::run<__nv_bfloat16, false>(ctx, a);
 }
