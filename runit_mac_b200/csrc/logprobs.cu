@@ -207,10 +207,10 @@ template <typename T, bool TOP> struct Pass {
     uint64_t z2 = 0, b2 = 0;                   // sums of 2^t and 2^t t since m has risen
 
     __device__ __forceinline__ void hand_over() {
-        const float e = fmaf(m, kLog2e, -r), f = exp2_approx(-e), zt = sum2(z2), bt = sum2(b2);
-        if (zt != 0.f) {                       // else nothing was added (and m need not be a number)
-            z = fmaf(f, zt, z);
-            b = fmaf(f * kLn2, fmaf(-e, zt, bt), b);
+        const float e = fmaf(m, kLog2e, -r), f = exp2_approx(-e), zs = sum2(z2), bs = sum2(b2);
+        if (zs != 0.f) {                       // else nothing was added (and m need not be a number)
+            z = fmaf(f, zs, z);
+            b = fmaf(f * kLn2, fmaf(-e, zs, bs), b);
         }
         z2 = b2 = 0;
     }
@@ -224,29 +224,38 @@ template <typename T, bool TOP> struct Pass {
         }
         if (__any_sync(0xffffffffu, !(all <= m) || !(fabsf(m) < Vec<T>::kFar))) {
             if (!rise(all)) {                  // no number, or far out
+#pragma unroll 1
+                for (int j = 0; j < V; j++) {
+                    uint4 x = u[0];
+                    float y = most[0];
 #pragma unroll
-                for (int j = 0; j < V; j++) plain(u[j], most[j], i + 32 * j);
+                    for (int q = 1; q < V; q++)
+                        if (q == j) { x = u[q]; y = most[q]; }
+                    plain(x, y, i + 32 * j);
+                }
                 return;
             }
-            if (leave) {                       // the entry goes where the floor is; it has been noted with its vector
+            if (leave) {                       // the entry goes where the floor is
 #pragma unroll
                 for (int j = 0; j < V; j++)
                     if (leave && most[j] == m) Vec<T>::drop(u[j], m, leave);
             }
         }
+#pragma unroll
+        for (int j = 0; j < V; j++) below(u[j], most[j], i + 32 * j);
+    }
+    // a vector below the maximum.  (Packed pairs are half the multiply-adds, on one of two pipes, and moves to form them: no gain.)
+    __device__ __forceinline__ void below(const uint4& u, float most, uint32_t i) {
+        if (TOP) note(most, i);
+        float v[N];
+        Vec<T>::raised(u, v);
         const uint64_t r2 = packf(-r), l2 = packf(kLog2e);
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-            if (TOP) note(most[j], i + 32 * j);
-            float v[N];
-            Vec<T>::raised(u[j], v);
-#pragma unroll
-            for (uint32_t e = 0; e < N; e += 2) {
-                const uint64_t t = ffma2(pack2(__float_as_uint(v[e]), __float_as_uint(v[e + 1])), l2, r2);
-                const uint64_t p = pack2(__float_as_uint(exp2_approx(__uint_as_float((uint32_t)t))), __float_as_uint(exp2_approx(__uint_as_float((uint32_t)(t >> 32)))));
-                z2 = fadd2(z2, p);
-                b2 = ffma2(p, t, b2);
-            }
+        for (uint32_t e = 0; e < N; e += 2) {
+            const uint64_t t = ffma2(pack2(__float_as_uint(v[e]), __float_as_uint(v[e + 1])), l2, r2);
+            const uint64_t p = pack2(__float_as_uint(exp2_approx(__uint_as_float((uint32_t)t))), __float_as_uint(exp2_approx(__uint_as_float((uint32_t)(t >> 32)))));
+            z2 = fadd2(z2, p);
+            b2 = ffma2(p, t, b2);
         }
     }
     __device__ __forceinline__ void note(float most, uint32_t i) {
@@ -332,8 +341,8 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
 }
 
 // A block takes rows blockIdx.x / cluster, + gridDim.x, ...; with few rows a cluster of `cluster` blocks (a power of two up to 16) shares one, and the first of them
-// adds up.  Seven warps read: each has a run of the row's 16-byte vectors, which come by bulk copies of 2 KB into its own ring of three, and goes on to its
-// run of the next row; the eighth warp turns what they have found into the row's results, one row behind.
+// adds up.  Seven warps read: the row's 16-byte vectors go to them in turn, 128 at a time, which come by a bulk copy of 2 KB into the warp's ring of three,
+// and a warp goes on to the next row when it is through; the eighth warp turns what they have found into the row's results, one row behind.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(const Args a, const uint32_t cluster) {
     constexpr uint32_t N = Vec<T>::N;
@@ -349,10 +358,10 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
     grid_dependency_wait();
     grid_launch_dependents();
     const uint32_t there = smem_u32(&bars[kWarps * kStages]), taken = there + 16;          // of the two buffers that hold a row's findings
-    // A row: entries ahead of the first 16-byte boundary, whole vectors, entries behind the last; the block's vectors v0 .. v1 - 1, a warp's `share`.
+    // A row: entries ahead of the first 16-byte boundary, whole vectors, entries behind the last; the block's vectors v0 .. v1 - 1.
     struct Run {
         const T* x;
-        uint32_t head, vecs, tail, v0, v1, share;
+        uint32_t head, vecs, tail, v0, v1;
     };
     auto run_of = [&](uint32_t row) {
         Run r;
@@ -363,7 +372,6 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
         const uint32_t per = (r.vecs + cluster - 1) / cluster;
         r.v0 = min(r.vecs, rank * per);
         r.v1 = min(r.vecs, r.v0 + per);
-        r.share = ((r.v1 - r.v0 + kWarps - 1) / kWarps + 31) / 32 * 32;
         return r;
     };
     bool ok = true;
@@ -373,32 +381,37 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
     if (warp < kWarps) {
         const uint4* const mine = reinterpret_cast<const uint4*>(ring + warp * kStages * kStageBytes);
         const uint32_t mine_s = smem_u32(mine), bar0 = smem_u32(&bars[warp * kStages]);
-        uint32_t asked = 0, used = 0;          // copies of this warp so far
-        // the run's copies that have been asked for go on into the next row's
-        uint32_t ask_row = blockIdx.x / cluster, ask_at = 0;
-        Run q = run_of(ask_row);
+        // The copies run ahead of the reading, on into the next row.  (What is kept here is what a copy costs least with:
+        // some 80 instructions for each of them were a quarter of all.)
+        uint32_t asked = 0, ask_slot = 0, slot = 0, phase = 0;
+        uint32_t ask_row = blockIdx.x / cluster, left = 0;
+        const uint4* next = nullptr;
+        auto enter = [&]() {                   // the run of ask_row
+            const Run q = run_of(ask_row);
+            left = q.v1 - q.v0 > warp * kStageVecs ? q.v1 - q.v0 - warp * kStageVecs : 0;
+            next = reinterpret_cast<const uint4*>(q.x + q.head) + q.v0 + warp * kStageVecs;
+        };
+        enter();
         auto ask = [&]() {
-            while (ask_row < a.rows) {
-                const uint32_t w0 = min(q.v1, q.v0 + warp * q.share), w1 = min(q.v1, w0 + q.share), v = w0 + ask_at;
-                if (v < w1) {
-                    if (lane == 0) {
-                        const uint32_t slot = asked % kStages, bar = bar0 + 8 * slot, bytes = 16 * min(kStageVecs, w1 - v);
-                        mbar_expect_tx(bar, bytes);
-                        bulk_load_1d(mine_s + slot * kStageBytes, reinterpret_cast<const uint4*>(q.x + q.head) + v, bytes, bar);
-                    }
-                    asked++;
-                    ask_at += kStageVecs;
-                    return;
-                }
-                ask_row += cluster > 1 ? a.rows : gridDim.x;
-                ask_at = 0;
-                if (ask_row < a.rows) q = run_of(ask_row);
+            while (left == 0) {
+                if (cluster > 1 || a.rows - ask_row <= gridDim.x) return;
+                ask_row += gridDim.x;
+                enter();
             }
+            const uint32_t n = min(left, kStageVecs);
+            if (lane == 0) {
+                mbar_expect_tx(bar0 + 8 * ask_slot, 16 * n);
+                bulk_load_1d(mine_s + ask_slot * kStageBytes, next, 16 * n, bar0 + 8 * ask_slot);
+            }
+            asked++;
+            ask_slot = ask_slot == kStages - 1 ? 0 : ask_slot + 1;
+            next += kWarps * kStageVecs;
+            left -= min(left, kWarps * kStageVecs);
         };
         for (uint32_t i = 0; i < kStages; i++) ask();
-        for (uint32_t row = blockIdx.x / cluster; row < a.rows; row += cluster > 1 ? a.rows : gridDim.x, turn++) {
+        for (uint32_t row = blockIdx.x / cluster;; turn++) {
             const Run r = run_of(row);
-            const uint32_t w0 = min(r.v1, r.v0 + warp * r.share), w1 = min(r.v1, w0 + r.share), half = turn & 1;
+            const uint32_t w0 = r.v0 + warp * kStageVecs, w1 = r.v1, half = turn & 1;
             Pass<T, TOP> pass;
             // up to N - 1 entries, one a lane
             auto few = [&](uint32_t first, uint32_t count) {
@@ -409,10 +422,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
                 pass.mine = was.mine; pass.second = was.second; pass.at = was.at; pass.nan = was.nan;
             };
             if (rank == 0 && warp == 0 && r.head) few(0, r.head);
-            for (uint32_t v = w0; v < w1; v += kStageVecs) {
-                const uint32_t slot = used % kStages;
+            for (uint32_t v = w0; v < w1; v += kWarps * kStageVecs) {
                 const uint4* const from = mine + slot * kStageVecs + lane;
-                if (ok) ok = __all_sync(0xffffffffu, wait(bar0 + 8 * slot, (used / kStages) & 1));
+                if (ok) ok = __all_sync(0xffffffffu, wait(bar0 + 8 * slot, phase));
                 uint4 u[kAhead];
                 if (v + kStageVecs <= w1) {
 #pragma unroll
@@ -421,7 +433,10 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
 #pragma unroll
                     for (uint32_t j = 0; j < kAhead; j++) u[j] = v + 32 * j + lane < w1 ? from[32 * j] : Vec<T>::nothing();
                 }
-                used++;
+                if (++slot == kStages) {
+                    slot = 0;
+                    phase ^= 1;
+                }
                 __syncwarp();
                 if (ok) ask();
                 pass.take(u, v + lane);
@@ -438,6 +453,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(there + 8 * half);
+            if (cluster > 1 || a.rows - row <= gridDim.x) break;
+            row += gridDim.x;
         }
         if (!ok) mbar_drain(bar0, kStages, asked);               // nothing is in flight when the block leaves
     }
@@ -460,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
         }
     };
     if (warp == kWarps) {
-        for (uint32_t row = blockIdx.x / cluster; row < a.rows; row += cluster > 1 ? a.rows : gridDim.x, turn++) {
+        for (uint32_t row = blockIdx.x / cluster;; turn++) {
             const Run r = run_of(row);
             const uint32_t half = turn & 1;
             if (ok) ok = __all_sync(0xffffffffu, wait(there + 8 * half, (turn / 2) & 1));
@@ -491,14 +508,17 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
                     for (uint32_t e = 0; e < N; e++) offer(v[e], vec, r.head + vec * N + e, in);
                 };
                 const bool mine = lane < a.k && t.v;
-                const uint32_t vec = ~t.i, run = mine ? (vec - r.v0) / r.share : 0, run0 = r.v0 + run * r.share, first = run0 + (vec - run0) % 32;
-                const bool whole = mine && ok && seconds[half][run][first - run0] >= least.v;
+                const uint32_t vec = ~t.i, of = mine ? (vec - r.v0) / kStageVecs % kWarps : 0, at = mine ? (vec - r.v0) % 32 : 0;
+                const bool whole = mine && ok && seconds[half][of][at] >= least.v;
                 offer_vector(vec, mine && ok && !whole);
                 uint32_t again = __ballot_sync(0xffffffffu, whole);
                 while (again) {
-                    const uint32_t from = __ffs(again) - 1, f = __shfl_sync(0xffffffffu, first, from), end = min(r.v1, __shfl_sync(0xffffffffu, run0, from) + r.share);
+                    const uint32_t from = __ffs(again) - 1, f = r.v0 + __shfl_sync(0xffffffffu, of * kStageVecs + at, from);
                     again &= again - 1;
-                    for (uint32_t j = f; j < end; j += 32 * 32) offer_vector(j + 32 * lane, j + 32 * lane < end);
+                    for (uint32_t j = lane; __any_sync(0xffffffffu, f + j / kAhead * kWarps * kStageVecs < r.v1); j += 32) {       // the lane's j-th vector
+                        const uint32_t v = f + j / kAhead * kWarps * kStageVecs + j % kAhead * 32;
+                        offer_vector(v, v < r.v1);
+                    }
                 }
                 // the entries outside of the vectors: those in front come before all others of their value, those behind after them
                 if (rank == 0 && r.head) offer(lane < r.head ? to_f32(r.x[lane]) : 0.f, 0, lane, lane < r.head);
@@ -511,6 +531,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
             __syncwarp();
             if (lane == 0) mbar_arrive(taken + 8 * half);
             if (cluster == 1) result(row);
+            if (cluster > 1 || a.rows - row <= gridDim.x) break;
+            row += gridDim.x;
         }
         if (cluster > 1) {
             if (lane == 0) all = s;
