@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
     float o[ND][4], m[2], l[2];
     // scores times mul are in units of log2; plain: products are scores times a positive scale.  Else they are scaled (before the cap or here) and biased.
     const bool plain = a.cap == 0.f && !a.slopes && a.scale > 0.f;
-    const float mul = plain ? a.scale * kLog2e : kLog2e, pre = a.cap != 0.f ? 1.f : a.scale, inv_cap = a.cap != 0.f ? 1.f / a.cap : 0.f;
+    const float mul = plain ? a.scale * kLog2e : kLog2e, pre = a.cap != 0.f ? a.cap : a.scale, to_cap = a.cap != 0.f ? a.scale / a.cap : 0.f;
     float slope[2];
     auto begin = [&]() {                       // rows of the reader's segment
 #pragma unroll
@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
             const bool all = __all_sync(0xffffffffu, inside);
             float top[2] = {-INFINITY, -INFINITY};
             if (!plain || !all) {
-                if (a.cap != 0.f) cap_scores(reinterpret_cast<float(&)[4 * NK]>(s), a.scale, a.cap, inv_cap);
+                if (a.cap != 0.f) tanh_scores(reinterpret_cast<float(&)[4 * NK]>(s), to_cap);
                 // in units of mul afterwards, like the plain ones
 #pragma unroll
                 for (uint32_t j = 0; j < NK; j++)

@@ -80,26 +80,33 @@ template <> struct Half2<__nv_bfloat16> {
 // the 16-bit halves of w that are no numbers, set to zero
 template <typename T> __device__ __forceinline__ uint32_t finite_part(uint32_t w, uint32_t nf) { return w & ~((nf >> 15) * 0xFFFFu); }
 
-// cap * tanh(scale v / cap) of N products, for a whole warp.  Below 0.35 tanh u = u (1 - u^2/3 + 2 u^4/15 - 17 u^6/315 + 62 u^8/2835), its Taylor series,
-// whose next term is 2.4e-7 of u there; a warp with a larger argument takes (1 - e^-2|u|) / (1 + e^-2|u|), off by some 2^-22 of the cap.
-template <int N> __device__ __forceinline__ void cap_scores(float (&v)[N], float scale, float cap, float inv_cap) {
+// tanh(k v) of N products, for a whole warp.  Below 0.35 tanh u = u (1 - u^2/3 + 2 u^4/15 - 17 u^6/315 + 62 u^8/2835), its Taylor series, whose next
+// term is 2.4e-7 of u there; a warp with a larger argument takes (1 - e^-2|u|) / (1 + e^-2|u|), off by some 2^-22.
+template <int N> __device__ __forceinline__ void tanh_scores(float (&v)[N], float k) {
+    uint64_t u[N / 2], w[N / 2];
+    const uint64_t k2 = packf(k), one = packf(1.f);
     float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        v[i] *= scale;
-        most = fmaxf(most, fabsf(v[i]));
+    for (int i = 0; i < N / 2; i++) {
+        u[i] = fmul2(pack2(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1])), k2);
+        w[i] = fmul2(u[i], u[i]);
+        most = fmaxf(most, fmaxf(__uint_as_float((uint32_t)w[i]), __uint_as_float((uint32_t)(w[i] >> 32))));
     }
-    if (__any_sync(0xffffffffu, most > 0.35f * cap)) {
+    if (__any_sync(0xffffffffu, most > 0.35f * 0.35f)) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const float e = exp2_approx(-2.f * kLog2e * fabsf(v[i]) * inv_cap);
-            v[i] = copysignf(cap * __fdividef(1.f - e, 1.f + e), v[i]);
+            const float x = v[i] * k, e = exp2_approx(-2.f * kLog2e * fabsf(x));
+            v[i] = copysignf(__fdividef(1.f - e, 1.f + e), x);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const float u = v[i] * inv_cap, w = u * u;
-            v[i] *= fmaf(w, fmaf(w, fmaf(w, fmaf(w, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+        for (int i = 0; i < N / 2; i++) {
+            uint64_t p = ffma2(w[i], packf(62.f / 2835.f), packf(-17.f / 315.f));
+            p = ffma2(w[i], p, packf(2.f / 15.f));
+            p = ffma2(w[i], p, packf(-1.f / 3.f));
+            p = fmul2(u[i], ffma2(w[i], p, one));
+            v[2 * i] = __uint_as_float((uint32_t)p);
+            v[2 * i + 1] = __uint_as_float((uint32_t)(p >> 32));
         }
     }
 }
