@@ -477,124 +477,139 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
     }
 }
 
-// Adds up what the launches have left of a (row, query head): a block for each.  First the factors 2^(m - max m) of all pieces, then the sums, the pieces
-// in turn over the block's warps, a lane 2 or 4 of the dimensions.  Rows that a worker has written itself are left.
+// Adds up what the launches have left of a (row, query head): a warp for each, or a block (WIDE) where a segment has many pieces.  A lane has the maximum and sum
+// of a piece, the factors 2^(m - max m) go round, and every lane adds up 2 or 4 of the dimensions.  Rows that a worker has written itself are left.
 struct MergeArgs {
     uint32_t n_entries;                        // of the split kernel: 0 when it has not run
     uint32_t own_parts, pre_parts;             // parts of the kernel for many rows: 0 when the split kernel has had those positions
     const float *own_o, *own_ml, *pre_o, *pre_ml;
     bool shared;
 };
-constexpr uint32_t kMaxPieces = kMaxWorkers + 640;
+constexpr uint32_t kMergeWarps = 8;
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(512) merge_kernel(const AttnArgs a, const MergeArgs g) {
+// Sequence of a row, by a warp: 33 parts at a time.
+__device__ __forceinline__ uint32_t sequence_by_warp(const Cache& c, uint32_t row) {
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t lo = 0, n = c.n_seqs;             // as many of q_start[1 ..] as are <= row: lo of them, and some of the n behind
+    while (n > 0) {
+        const uint32_t step = n / 33 + 1, at = lo + (lane + 1) * step;
+        const uint32_t hit = __popc(__ballot_sync(0xffffffffu, at <= lo + n && c.q_start[at] <= (int32_t)row));
+        const uint32_t end = lo + n;
+        lo += hit * step;
+        n = min(step - 1, end - lo);
+    }
+    return lo;
+}
+
+template <typename T, int HD, bool WIDE>
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttnArgs a, const MergeArgs g) {
     constexpr uint32_t E = HD / 32;
     grid_dependency_wait();
     grid_launch_dependents();
-    __shared__ float factor[kMaxPieces], red[2][16], so[16][HD];
     const Cache& c = a.c;
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5, head = blockIdx.x % c.heads, token = blockIdx.x / c.heads;
-    const uint32_t s = sequence_by_halves(c, token);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint64_t pairs = (uint64_t)c.rows * c.heads, orow = WIDE ? blockIdx.x : (uint64_t)blockIdx.x * kMergeWarps + warp;
+    if (orow >= pairs) return;
+    const uint32_t token = (uint32_t)(orow / c.heads), head = (uint32_t)(orow % c.heads);
+    const uint32_t s = sequence_by_warp(c, token);
     if (s >= c.n_seqs) return;
-    const size_t orow = (size_t)token * c.heads + head, pairs = (size_t)c.rows * c.heads;
+    const Seq q = sequence(c, s);
+    if (token < q.row0 || token >= q.row0 + q.n) return;
     // pieces of one entry: as many, from worker w0 on, or one that is whole
     struct List {
         uint32_t n, w0, beg, row;
-        bool whole;
     };
     uint32_t workers = 1, total = 0;
     auto list_of = [&](const Entry& u, uint32_t e, uint32_t i) {
-        List x{0, 0, 0, i % kRows, false};
+        List x{0, 0, 0, i % kRows};
         if (u.steps == 0) return x;
         x.beg = a.plan[kPlanHead + e] + (head / c.group * u.tiles + i / kRows) * u.steps;
         x.w0 = owner_of(x.beg, total, workers);
         x.n = owner_of(x.beg + u.steps - 1, total, workers) - x.w0 + 1;
-        x.whole = x.n == 1;
         return x;
     };
-    List own{g.own_parts, 0, 0, 0, false}, pre{g.pre_parts, 0, 0, 0, false};
-    const Seq q = sequence(c, s);
-    if (token < q.row0 || token >= q.row0 + q.n) return;
+    List own{g.own_parts, 0, 0, 0}, pre{g.pre_parts, 0, 0, 0};
     if (g.n_entries) {
         const uint32_t pre_lo = a.plan[0], pre_hi = a.plan[1], e0 = a.plan[3];
         workers = a.plan[2];
         total = a.plan[4];
         if (!g.own_parts) {
             own = list_of(entry_of(a, s, pre_lo, pre_hi), s - e0, (token - q.row0) * c.group + head % c.group);
-            if (own.whole && !g.shared) return;
+            if (own.n == 1 && !g.shared) return;
         }
         if (g.shared && !g.pre_parts) pre = list_of(entry_of(a, c.n_seqs, pre_lo, pre_hi), c.n_seqs - e0, token * c.group + head % c.group);
     }
-    const uint32_t n = own.n + pre.n;
-    auto piece = [&](uint32_t i, const float** po) -> const float* {
-        const bool p = i >= own.n;
-        const List& x = p ? pre : own;
-        if (p) i -= own.n;
-        if (p ? g.pre_parts : g.own_parts) {
-            *po = (p ? g.pre_o : g.own_o) + (i * pairs + orow) * HD;
-            return (p ? g.pre_ml : g.own_ml) + (i * pairs + orow) * 2;
-        }
-        if (x.whole) {
-            *po = (p ? a.pre_o : a.row_o) + orow * HD;
-            return (p ? a.pre_ml : a.row_ml) + orow * 2;
-        }
-        const Piece s = slot_of(a, x.w0 + i, begin_of(x.w0 + i, total, workers) >= x.beg);
-        *po = s.o + x.row * HD;
-        return s.ml + x.row * 2;
-    };
-    auto over_block = [&](float v, bool most, float* r) {
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
-            const float t = __shfl_xor_sync(0xffffffffu, v, d);
-            v = most ? fmaxf(v, t) : v + t;
-        }
-        if (warps == 1) return v;
-        if (lane == 0) r[warp] = v;
-        __syncthreads();
-        v = r[0];
-        for (uint32_t w = 1; w < warps; w++) v = most ? fmaxf(v, r[w]) : v + r[w];
-        return v;
-    };
+    const uint32_t n = own.n + pre.n, step = WIDE ? kMergeWarps : 1;
     float m = -INFINITY, l = 0.f, o[E];
-    for (uint32_t i = tid; i < n; i += blockDim.x) {
-        const float* po;
-        const float x = piece(i, &po)[0];
-        factor[i] = x;
-        m = fmaxf(m, x);
-    }
-    m = over_block(m, true, red[0]);
-    for (uint32_t i = tid; i < n; i += blockDim.x) {
-        const float* po;
-        const float f = m == -INFINITY ? 1.f : exp2_approx(factor[i] - m);         // no score at all: the sums are 0, or no numbers
-        factor[i] = f;
-        l = fmaf(f, piece(i, &po)[1], l);
-    }
-    l = over_block(l, false, red[1]);
-    __syncwarp();
 #pragma unroll
     for (uint32_t e = 0; e < E; e++) o[e] = 0.f;
-#pragma unroll 4
-    for (uint32_t i = warp; i < n; i += warps) {
-        const float* po;
-        piece(i, &po);
-        const float f = factor[i];
-        if constexpr (E == 4) {
-            const float4 x = *reinterpret_cast<const float4*>(po + 4 * lane);
-            o[0] = fmaf(f, x.x, o[0]); o[1] = fmaf(f, x.y, o[1]); o[2] = fmaf(f, x.z, o[2]); o[3] = fmaf(f, x.w, o[3]);
-        } else {
-            const float2 x = *reinterpret_cast<const float2*>(po + 2 * lane);
-            o[0] = fmaf(f, x.x, o[0]); o[1] = fmaf(f, x.y, o[1]);
+    for (uint32_t i0 = WIDE ? warp : 0; i0 < n; i0 += 32 * step) {           // a warp's pieces i0, i0 + step, ...: 32 at a time
+        uint32_t i = i0 + lane * step;
+        const uint32_t count = min(32u, (n - i0 + step - 1) / step);
+        const float *po = a.slot_o, *pml = nullptr;
+        if (i < n) {
+            const bool p = i >= own.n;
+            const List& x = p ? pre : own;
+            if (p) i -= own.n;
+            if (p ? g.pre_parts : g.own_parts) {
+                po = (p ? g.pre_o : g.own_o) + (i * pairs + orow) * HD;
+                pml = (p ? g.pre_ml : g.own_ml) + (i * pairs + orow) * 2;
+            } else if (x.n == 1) {
+                po = (p ? a.pre_o : a.row_o) + orow * HD;
+                pml = (p ? a.pre_ml : a.row_ml) + orow * 2;
+            } else {
+                const Piece y = slot_of(a, x.w0 + i, begin_of(x.w0 + i, total, workers) >= x.beg);
+                po = y.o + x.row * HD;
+                pml = y.ml + x.row * 2;
+            }
+        }
+        const float2 ml = pml ? *reinterpret_cast<const float2*>(pml) : make_float2(-INFINITY, 0.f);
+        float top = fmaxf(m, ml.x);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        // no score at all: the sums are 0, or no numbers
+        const float f = !pml ? 0.f : top == -INFINITY ? 1.f : exp2_approx(ml.x - top), old = top == -INFINITY ? 1.f : exp2_approx(m - top);
+        float sum = pml ? f * ml.y : 0.f;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        l = fmaf(l, old, sum);
+        m = top;
+#pragma unroll
+        for (uint32_t e = 0; e < E; e++) o[e] *= old;
+        const uint64_t at = reinterpret_cast<uint64_t>(po);
+#pragma unroll 8
+        for (uint32_t k = 0; k < count; k++) {
+            const float* x = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, at, k));
+            const float fk = __shfl_sync(0xffffffffu, f, k);
+            if constexpr (E == 4) {
+                const float4 v = *reinterpret_cast<const float4*>(x + 4 * lane);
+                o[0] = fmaf(fk, v.x, o[0]); o[1] = fmaf(fk, v.y, o[1]); o[2] = fmaf(fk, v.z, o[2]); o[3] = fmaf(fk, v.w, o[3]);
+            } else {
+                const float2 v = *reinterpret_cast<const float2*>(x + 2 * lane);
+                o[0] = fmaf(fk, v.x, o[0]); o[1] = fmaf(fk, v.y, o[1]);
+            }
         }
     }
-    if (warps > 1) {
+    if constexpr (WIDE) {
+        __shared__ float sm[kMergeWarps], sl[kMergeWarps], so[kMergeWarps][HD];
+        if (lane == 0) { sm[warp] = m; sl[warp] = l; }
 #pragma unroll
         for (uint32_t e = 0; e < E; e++) so[warp][E * lane + e] = o[e];
         __syncthreads();
         if (warp > 0) return;
-        for (uint32_t w = 1; w < warps; w++)
+        float top = m;
 #pragma unroll
-            for (uint32_t e = 0; e < E; e++) o[e] += so[w][E * lane + e];
+        for (uint32_t w = 1; w < kMergeWarps; w++) top = fmaxf(top, sm[w]);
+        l = 0.f;
+#pragma unroll
+        for (uint32_t e = 0; e < E; e++) o[e] = 0.f;
+#pragma unroll
+        for (uint32_t w = 0; w < kMergeWarps; w++) {
+            const float f = top == -INFINITY ? 1.f : exp2_approx(sm[w] - top);
+            l = fmaf(f, sl[w], l);
+#pragma unroll
+            for (uint32_t e = 0; e < E; e++) o[e] = fmaf(f, so[w][E * lane + e], o[e]);
+        }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + (size_t)token * a.ldo + (size_t)head * HD);
@@ -701,10 +716,11 @@ static int32_t run(runit_ctx* ctx, const runit_paged_cfg* g, const runit_paged_b
         share = grid * kWarps / max(1u, c.n_entries * g->kv_heads);
     }
     if (c.direct) return RUNIT_OK;
-    // warps of a merging block: about a quarter of the pieces that a segment has when all are alike
-    const uint32_t warps = share >= 32 ? 16 : share >= 16 ? 8 : share >= 4 ? 4 : 1;
     const MergeArgs m{c.n_entries, c.own_tc ? c.own_split : 0, c.pre_tc ? c.pre_split : 0, own.part_o, own.part_ml, pre.part_o, pre.part_ml, b->shared_len != 0};
-    runit_launch_chain(ctx, merge_kernel<T, HD>, dim3(g->heads * b->rows), dim3(32 * warps), a, m);
+    // a block for each where a segment has more pieces than a warp asks for at once, when all are alike
+    const uint64_t pairs = (uint64_t)g->heads * b->rows;
+    if (share >= 16) runit_launch_chain(ctx, merge_kernel<T, HD, true>, dim3((uint32_t)pairs), dim3(kMergeWarps * 32), a, m);
+    else runit_launch_chain(ctx, merge_kernel<T, HD, false>, dim3((uint32_t)((pairs + kMergeWarps - 1) / kMergeWarps)), dim3(kMergeWarps * 32), a, m);
     return runit_after_launch(ctx, "paged_attention (merge)");
 }
 
