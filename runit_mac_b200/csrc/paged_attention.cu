@@ -15,6 +15,7 @@ namespace pg {
 constexpr uint32_t kWarps = 4, kStep = 32, kBox = 16, kRows = 16, kPlanHead = 16;
 constexpr uint32_t kMaxWorkers = kWarps * 256;
 constexpr uint32_t kStepsMin = 2;              // a worker's share at least: what it costs to begin and to merge is that of about two steps
+constexpr uint32_t kFew = 256;                 // up to so many entries every warp finds its place for itself, without meeting the others
 
 template <int HD> struct Shape {
     static constexpr uint32_t kBoxBytes = kBox * HD * 2, kStage = 4 * kBoxBytes, kStages = HD == 128 ? 3 : 6;
@@ -28,7 +29,9 @@ struct Entry {
     int32_t base;                              // position of its first row
     const int32_t* table;
 };
-__device__ __forceinline__ uint32_t steps_of(uint32_t lo, uint32_t hi) { return hi > lo ? (hi - (lo & ~(kBox - 1)) + kStep - 1) / kStep : 0; }
+// One more than its positions take: beginning and ending a segment costs a worker 1.5 steps (64 sequences of 60 to 8100 positions: 113000 clocks for those
+// with eight segments, 83000 for those with one).
+__device__ __forceinline__ uint32_t steps_of(uint32_t lo, uint32_t hi) { return hi > lo ? (hi - (lo & ~(kBox - 1)) + kStep - 1) / kStep + 1 : 0; }
 __device__ __forceinline__ Entry entry_of(const AttnArgs& a, uint32_t e, uint32_t pre_lo, uint32_t pre_hi) {
     const Cache& c = a.c;
     Entry t;
@@ -52,9 +55,12 @@ __device__ __forceinline__ Entry entry_of(const AttnArgs& a, uint32_t e, uint32_
     t.steps = steps_of(t.lo, t.hi);
     return t;
 }
-// Worker w of `workers` has the steps from begin_of(w) to begin_of(w + 1).
-__device__ __forceinline__ uint32_t begin_of(uint32_t w, uint32_t total, uint32_t workers) { return (uint32_t)((uint64_t)w * total / workers); }
-__device__ __forceinline__ uint32_t owner_of(uint32_t step, uint32_t total, uint32_t workers) { return (uint32_t)((((uint64_t)step + 1) * workers - 1) / total); }
+// Worker w of `workers` has the steps from begin_of(w) to begin_of(w + 1): the first ones have one more than the others.
+__device__ __forceinline__ uint32_t begin_of(uint32_t w, uint32_t total, uint32_t workers) { return w * (total / workers) + min(w, total % workers); }
+__device__ __forceinline__ uint32_t owner_of(uint32_t step, uint32_t total, uint32_t workers) {
+    const uint32_t each = total / workers, more = total % workers, mid = more * (each + 1);
+    return step < mid ? step / (each + 1) : more + (step - mid) / each;
+}
 __device__ __forceinline__ uint32_t workers_of(uint32_t total, uint32_t most) { return max(1u, min(most, total / kStepsMin)); }
 
 struct Piece {
@@ -122,56 +128,99 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
     __syncthreads();
     grid_dependency_wait();
     grid_launch_dependents();
-    // the shared positions that some row sees
-    if (e0 + n_entries > c.n_seqs) {
-        uint32_t lo = c.shared, hi = 0;
-        for (uint32_t e = tid; e < c.n_seqs; e += kWarps * 32) {
-            const Seq s = sequence(c, e);
-            if (!s.n) continue;
-            lo = min(lo, first_seen((int32_t)s.len - (int32_t)s.n, a.window));
-            hi = max(hi, min(s.len, c.shared));
+    uint32_t pre_lo = c.shared, pre_hi = 0, total = 0, workers, me = warp * gridDim.x + blockIdx.x, x0, x1, e_first = 0, e_before = 0;
+    // neighbours in the order of steps sit on other SMs: few steps spread over all of them
+    auto share = [&]() {
+        workers = workers_of(total, gridDim.x * kWarps);
+        x0 = me < workers && total ? begin_of(me, total, workers) : 0;
+        x1 = me < workers && total ? begin_of(me + 1, total, workers) : 0;
+    };
+    auto seen = [&](uint32_t e) {              // the shared positions that some row of a sequence sees
+        const Seq s = sequence(c, e);
+        if (!s.n) return;
+        pre_lo = min(pre_lo, first_seen((int32_t)s.len - (int32_t)s.n, a.window));
+        pre_hi = max(pre_hi, min(s.len, c.shared));
+    };
+    auto cost = [&](uint32_t e) {
+        const Entry t = entry_of(a, e0 + e, pre_lo, pre_hi);
+        return t.tiles * t.steps * c.kv_heads;
+    };
+    auto scan = [&](uint32_t v) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= (uint32_t)o) v += u;
         }
-        atomicMin(&edge[0], lo);
-        atomicMax(&edge[1], hi);
-        __syncthreads();
-    }
-    const uint32_t pre_lo = edge[0], pre_hi = edge[1];
-    {
+        return v;
+    };
+    const bool with_pre = e0 + n_entries > c.n_seqs;
+    if (n_entries <= kFew) {
+        if (with_pre) {
+            for (uint32_t e = lane; e < c.n_seqs; e += 32) seen(e);
+            pre_lo = __reduce_min_sync(0xffffffffu, pre_lo);
+            pre_hi = __reduce_max_sync(0xffffffffu, pre_hi);
+        }
+        // (not unrolled: what a warp runs once costs most where its instructions come from)
+#pragma unroll 1
+        for (uint32_t k = 0; k < n_entries; k += 32) total += __reduce_add_sync(0xffffffffu, k + lane < n_entries ? cost(k + lane) : 0);
+        share();
+        uint32_t at = 0;
+#pragma unroll 1
+        for (uint32_t k = 0; k < n_entries; k += 32) {
+            const uint32_t v = k + lane < n_entries ? cost(k + lane) : 0, inc = scan(v) + at;
+            if (blockIdx.x == 0 && warp == 0 && k + lane < n_entries) a.plan[kPlanHead + k + lane] = inc - v;
+            const uint32_t here = __ballot_sync(0xffffffffu, v && x0 >= inc - v && x0 < inc);
+            if (here) {
+                e_first = k + __ffs(here) - 1;
+                e_before = __shfl_sync(0xffffffffu, inc - v, __ffs(here) - 1);
+            }
+            at = __shfl_sync(0xffffffffu, inc, 31);
+        }
+    } else {
+        if (with_pre) {
+            for (uint32_t e = tid; e < c.n_seqs; e += kWarps * 32) seen(e);
+            atomicMin(&edge[0], pre_lo);
+            atomicMax(&edge[1], pre_hi);
+            __syncthreads();
+            pre_lo = edge[0];
+            pre_hi = edge[1];
+        }
         const uint32_t per = (n_entries + kWarps * 32 - 1) / (kWarps * 32), beg = min(n_entries, tid * per), end = min(n_entries, beg + per);
         uint32_t sum = 0;
         for (uint32_t e = beg; e < end; e++) {
-            const Entry t = entry_of(a, e0 + e, pre_lo, pre_hi);
             before[e] = sum;
-            sum += t.tiles * t.steps * c.kv_heads;
+            sum += cost(e);
         }
-        uint32_t inc = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= (uint32_t)o) inc += v;
-        }
+        const uint32_t inc = scan(sum);
         if (lane == 31) sums[warp] = inc;
         __syncthreads();
         uint32_t off = inc - sum;
         for (uint32_t w = 0; w < warp; w++) off += sums[w];
-        for (uint32_t e = beg; e < end; e++) before[e] += off;
+        for (uint32_t e = beg; e < end; e++) {
+            before[e] += off;
+            if (blockIdx.x == 0) a.plan[kPlanHead + e] = before[e];
+        }
         if (tid == kWarps * 32 - 1) before[n_entries] = off + sum;
         __syncthreads();
-    }
-    const uint32_t total = before[n_entries], workers = workers_of(total, gridDim.x * kWarps);
-    if (blockIdx.x == 0) {
-        for (uint32_t e = tid; e <= n_entries; e += kWarps * 32) a.plan[kPlanHead + e] = before[e];
-        if (tid == 0) {
-            a.plan[0] = pre_lo;
-            a.plan[1] = pre_hi;
-            a.plan[2] = workers;
-            a.plan[3] = e0;
-            a.plan[4] = total;
+        total = before[n_entries];
+        share();
+        uint32_t l = 0, r = n_entries;         // the last entry that begins at or before x0 (those without steps come before it)
+        while (r - l > 1) {
+            const uint32_t mid = (l + r) / 2;
+            if (before[mid] <= x0) l = mid;
+            else r = mid;
         }
+        e_first = l;
+        e_before = before[l];
     }
-    const uint32_t me = warp * gridDim.x + blockIdx.x;          // neighbours in the order of steps sit on other SMs: few steps spread over all of them
-    if (me >= workers || total == 0) return;
-    const uint32_t x0 = begin_of(me, total, workers), x1 = begin_of(me + 1, total, workers);
+    if (blockIdx.x == 0 && tid == 0) {
+        a.plan[0] = pre_lo;
+        a.plan[1] = pre_hi;
+        a.plan[2] = workers;
+        a.plan[3] = e0;
+        a.plan[4] = total;
+    }
+    if (x0 == x1) return;
 
     // A place in the order of steps.  Reader and copier walk it, the copier kStages ahead.
     struct Cursor {
@@ -188,21 +237,6 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
             u.lo = max(u.lo, first_seen(p0, a.window));
         }
     };
-    auto seek = [&](Cursor& u, uint32_t x) {
-        uint32_t l = 0, r = n_entries;         // the last entry that begins at or before x and is not empty
-        while (r - l > 1) {
-            const uint32_t mid = (l + r) / 2;
-            if (before[mid] <= x) l = mid;
-            else r = mid;
-        }
-        u.e = e0 + l;
-        u.t = entry_of(a, u.e, pre_lo, pre_hi);
-        const uint32_t at = x - before[l], seg = at / u.t.steps;
-        u.h = seg / u.t.tiles;
-        u.tile = seg % u.t.tiles;
-        u.step = at % u.t.steps;
-        enter(u);
-    };
     auto next = [&](Cursor& u, uint32_t x) {   // to step x, the one behind
         if (++u.step < u.t.steps) return;
         u.step = 0;
@@ -211,8 +245,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
             if (++u.h == c.kv_heads) {
                 u.h = 0;
                 if (x >= total) return;
-                do u.e++;
-                while (before[u.e - e0 + 1] <= x);
+                uint32_t some = 0;             // the next entry that has steps (there is one)
+                for (u.e++; !(some = __ballot_sync(0xffffffffu, u.e - e0 + lane < n_entries && cost(u.e - e0 + lane))) && u.e - e0 < n_entries; u.e += 32) {}
+                u.e += __ffs(some) - 1;
                 u.t = entry_of(a, u.e, pre_lo, pre_hi);
             }
         }
@@ -223,22 +258,39 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
 
     const uint32_t bar0 = smem_u32(&bars[warp * S::kStages]), ring0 = smem_u32(ring) + warp * S::kStages * S::kStage;
     Cursor in, at;
-    seek(at, x0);
+    at.e = e0 + e_first;
+    at.t = entry_of(a, at.e, pre_lo, pre_hi);
+    {
+        const uint32_t of = x0 - e_before, seg = of / at.t.steps;
+        at.h = seg / at.t.tiles;
+        at.tile = seg % at.t.tiles;
+        at.step = of % at.t.steps;
+        enter(at);
+    }
     in = at;
-    int32_t page[2];
-    auto look_up = [&]() {                     // pages of the copier's next step
-        const uint32_t k = key_of(in);
-#pragma unroll
-        for (uint32_t b = 0; b < 2; b++) page[b] = k + b * kBox < in.hi ? in.t.table[(k + b * kBox) >> c.page_log2] : 0;
+    // pages of the next 32 boxes of the copier's segment, one a lane
+    int32_t pages = 0;
+    uint32_t pages_at = 0;                     // the step whose boxes come first
+    auto look_up = [&]() {
+        const uint32_t k = key_of(in) + lane * kBox;
+        pages = k < in.hi ? in.t.table[k >> c.page_log2] : 0;
+        pages_at = in.step;
+    };
+    auto advance = [&](uint32_t x) {
+        next(in, x);
+        if (in.step == 0 || in.step == pages_at + 16) look_up();
     };
     auto copy = [&](uint32_t stage) {
         const uint32_t k = key_of(in), n = hidden(in) ? 0 : k + kBox < in.hi ? 2 : 1;
+        int32_t page[2];
 #pragma unroll
-        for (uint32_t b = 0; b < 2; b++)
+        for (uint32_t b = 0; b < 2; b++) {
+            page[b] = __shfl_sync(0xffffffffu, pages, 2 * (in.step - pages_at) + b);
             if (b < n && (uint32_t)page[b] >= c.n_pages) {
                 report(c);
                 page[b] = 0;
             }
+        }
         if (lane == 0) {
             const uint32_t bar = bar0 + 8 * stage, dst = ring0 + stage * S::kStage;
             mbar_expect_tx(bar, n * 2 * S::kBoxBytes);
@@ -255,12 +307,6 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
     };
     uint32_t xin = x0;
     look_up();
-    for (uint32_t s = 0; s < S::kStages && xin < x1; s++) {
-        copy(s);
-        xin++;
-        next(in, xin);
-        if (xin < x1) look_up();
-    }
 
     uint32_t qa[KS][4], lo[2], hi[2];
     int32_t pos[2];
@@ -339,6 +385,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
     bool ok = true;
     uint32_t begun = x0 - at.step;             // where the segment begins in the order of steps
     begin();
+    for (uint32_t s = 0; s < S::kStages && xin < x1; s++) {
+        copy(s);
+        xin++;
+        if (xin < x1) advance(xin);
+    }
     for (uint32_t x = x0; x < x1 && ok; x++) {
         const uint32_t n = x - x0, stage = n % S::kStages;
         ok = __all_sync(0xffffffffu, mbar_wait(bar0 + 8 * stage, (n / S::kStages) & 1));
@@ -347,18 +398,27 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
         if (!hidden(at)) {
             const uint32_t sk = ring0 + stage * S::kStage, sv = sk + 2 * S::kBoxBytes;
             float s[NK][4];
+            uint32_t row_at[NK];                   // a lane's place among the rows of keys 8 j .. 8 j + 7
 #pragma unroll
             for (uint32_t j = 0; j < NK; j++) {
                 s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-                const uint32_t row = (j & 1) * 8 + (lane & 7);
+                row_at[j] = sk + (j >> 1) * S::kBoxBytes + ((j & 1) * 8 + (lane & 7)) * 128;
+            }
+            // products of four blocks of keys next to each other, none of which waits for another
+            uint32_t b[2][NK][4];
+            auto keys = [&](uint32_t k, uint32_t (&x)[NK][4]) {
+                const uint32_t ch = 2 * k + (lane >> 3);                            // 16-byte piece of the key's row
 #pragma unroll
-                for (uint32_t k = 0; k < KS; k += 2) {
-                    uint32_t b[4];
-                    const uint32_t ch = 2 * k + (lane >> 3);                        // 16-byte piece of the key's row
-                    ldsm_x4(b, sk + (j >> 1) * S::kBoxBytes + (ch >> 3) * (kBox * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
-                    Half2<T>::mma(s[j], qa[k], b[0], b[1]);
-                    Half2<T>::mma(s[j], qa[k + 1], b[2], b[3]);
-                }
+                for (uint32_t j = 0; j < NK; j++) ldsm_x4(x[j], row_at[j] + (ch >> 3) * (kBox * 128) + (((ch & 7) ^ (lane & 7)) << 4));
+            };
+            keys(0, b[0]);
+#pragma unroll
+            for (uint32_t k = 0; k < KS; k += 2) {
+                if (k + 2 < KS) keys(k + 2, b[(k / 2 + 1) & 1]);
+#pragma unroll
+                for (uint32_t j = 0; j < NK; j++) Half2<T>::mma(s[j], qa[k], b[(k / 2) & 1][j][0], b[(k / 2) & 1][j][1]);
+#pragma unroll
+                for (uint32_t j = 0; j < NK; j++) Half2<T>::mma(s[j], qa[k + 1], b[(k / 2) & 1][j][2], b[(k / 2) & 1][j][3]);
             }
             // a thread has keys 8 j + 2 t4, + 1 of rows g4 and g4 + 8
             const bool inside = k0 >= lo[0] && k0 >= lo[1] && k0 + kStep <= hi[0] && k0 + kStep <= hi[1];
@@ -460,8 +520,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
         if (xin < x1) {
             copy(stage);
             xin++;
-            next(in, xin);
-            if (xin < x1) look_up();
+            if (xin < x1) advance(xin);
         }
         const uint32_t left = at.t.steps - at.step - 1;
         if (left == 0 || x + 1 == x1) {
