@@ -2,8 +2,9 @@
 //
 // A CTA has up to 256 (row, query head) pairs of one key head, as two tiles of 128, and walks a part of their positions in blocks of 128 that both tiles
 // share.  A tile's block: S = Q K^T into tensor memory (f32); four warps, a thread a row, take the maximum of S, form the weights 2^(s - ref) and put
-// them down as 16-bit numbers in the columns of S, 64 positions and then the others, each handed over for itself; O += P V, accumulated in tensor memory, P
-// being the A operand from there and V (as it lies in the cache) MN-major.  The products of one tile run under the exponentials of the other.  ref is a row's largest score until one exceeds it by 2^8, so that O
+// them down as 16-bit numbers in columns of S that have been read; O += P V, accumulated in tensor memory, P being the A operand from there and V (as
+// it lies in the cache) MN-major.  That goes by halves of a block, 64 positions, each with columns of its own: while the weights of one are formed, the scores
+// of the next one are there already, and the products of the last one run (whole blocks: 3900 clocks a block of both tiles, halves 3700).  ref is a row's largest score until one exceeds it by 2^8, so that O
 // is rarely scaled; weights up to 2^8 keep the relative error of their rounding, and sums of them are f32.
 // Bound: exponentials (16 a clock and SM) and products (4096 multiply-adds a clock and SM) both take 2048 clocks for 256 rows x 128 positions x dim 128.
 // K and V of a block come by TMA as boxes of whole pages or of 128 positions; positions outside of what the CTA's rows see are zeros in V.
@@ -35,16 +36,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        uint32_t v[16];
-#pragma unroll
-        for (int j = 0; j < 16; j++) v[j] = r[16 * h + j];
-        tmem_st16(taddr + 16 * h, v);
-    }
-}
-
 // One row's attention over positions lo .. hi of a table, by a warp with plain arithmetic: for rows whose products met a value that is no number at a
 // position that they do not see (0 x Inf).  Returns maximum (log2 units) and sum; o: HD / 32 of the dimensions per lane.
 template <typename T, int HD>
@@ -83,14 +74,14 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const AttnArgs a, const TcArgs w) {
     using S = TcShape<HD>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * S::kSlots + 10];
+    __shared__ __align__(8) uint64_t bars[2 * S::kSlots + 12];
     __shared__ uint32_t tmem_holder, found[4], sums[kTcThreads / 32];
     __shared__ volatile int abort_flag;
     const Cache& c = a.c;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    // full, empty: one phase per use of a slot; s_full, p_full (two halves), turn: one per block of a tile; done: one
-    const uint32_t full = smem_u32(bars), empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots, p_full = s_full + 16, done = p_full + 32, turn = done + 16;
+    // full, empty: one phase per use of a slot; s_full, p_full of a tile's halves: one per block; o_full: one per half block; done: one
+    const uint32_t full = smem_u32(bars), empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots, p_full = s_full + 32, o_full = p_full + 32, done = o_full + 16;
     if (tid == 0) {
         abort_flag = 0;
         found[0] = 0xFFFFFFFFu;
@@ -202,11 +193,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
             mbar_init(empty + 8 * i, chains);
         }
         for (uint32_t i = 0; i < 2; i++) {
-            mbar_init(s_full + 8 * i, 1);
+            mbar_init(o_full + 8 * i, 1);
             mbar_init(done + 8 * i, 1);
-            mbar_init(turn + 8 * i, 4);
-            mbar_init(p_full + 16 * i, 128);
-            mbar_init(p_full + 16 * i + 8, 128);
+        }
+        for (uint32_t i = 0; i < 4; i++) {
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(p_full + 8 * i, 128);
         }
         fence_mbar_init();
     }
@@ -240,7 +232,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
         mbar_drain(full, S::kSlots, n);
     } else if (warp >= kSoftWarps) {           // a tile's products
         const uint32_t i = warp - kSoftWarps, qs = base + i * S::kTile, s_cols = tmem + 128 * i, o_cols = tmem + 256 + 128 * i;
-        uint32_t n_s = 0, n_d = 0;
+        const uint32_t halves = i < chains ? 2 * n_blocks : 0;
+        uint32_t n_s[2] = {0, 0}, n_o = 0, n_d = 0;
         auto slot_of_use = [&](uint32_t n) { return base + (2 + n % S::kSlots) * S::kTile; };
         auto wait = [&](uint32_t bar, uint32_t parity) {
             ok = ok && mbar_wait_timed(bar, parity, &abort_flag);
@@ -248,62 +241,68 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
             tc_fence_after_sync();
         };
         auto wait_full = [&](uint32_t n) { wait(full + 8 * (n % S::kSlots), (n / S::kSlots) & 1); };
-        auto scores = [&](uint32_t n) {        // with the block of K that is use n; the slot is free behind them
-            const uint32_t kb = slot_of_use(n);
+        // half h of a block's scores, with the block of K that is use n; the slot is free behind the second one
+        auto scores = [&](uint32_t n, uint32_t h) {
+            const uint32_t kb = slot_of_use(n) + 8192 * h;
             if (elect_one()) {
 #pragma unroll
                 for (int s = 0; s < HD / 16; s++) {
                     const uint32_t off = (s >> 2) * S::kPanel + (s & 3) * 32;
-                    umma_bf16(s_cols, umma_desc_sw128(qs + off), umma_desc_sw128(kb + off), idesc_of<T>(128, kKeys, 0), s > 0);
+                    umma_bf16(s_cols + 64 * h, umma_desc_sw128(qs + off), umma_desc_sw128(kb + off), idesc_of<T>(128, kKeys / 2, 0), s > 0);
                 }
-                umma_commit(s_full + 8 * i);
-                umma_commit(empty + 8 * (n % S::kSlots));
+                umma_commit(s_full + 16 * i + 8 * h);
+                if (h) umma_commit(empty + 8 * (n % S::kSlots));
             }
             __syncwarp();
-            n_s++;
+            n_s[h]++;
         };
         asm volatile("bar.sync 1, 320;" ::: "memory");           // Q is there
         tc_fence_after_sync();
-        if (i < chains && n_blocks > 0) {
+        if (halves) {
             wait_full(0);
-            if (ok) scores(0);
+            if (ok) scores(0, 0);
+            if (ok) scores(0, 1);
         }
-        for (uint32_t j = 0; j < (i < chains ? n_blocks : 0) && ok; j++) {
-            const bool last = j + 1 == n_blocks;
-            const uint32_t uv = 2 * j + 1, uk = 2 * j + 2, k0 = start + (b0 + j) * kKeys, vb = slot_of_use(uv);
-            wait_full(uv);
-            if (!ok) break;
-            if (k0 < lo || k0 + kKeys > hi) {  // zeros where no row looks: the copies have left there what lay there, or the neighbours of what was asked for
-                const uint32_t from = lo > k0 ? lo - k0 : 0, to = hi - k0;
-                for (uint32_t x = lane; x < kKeys * (HD / 8); x += 32) {
-                    const uint32_t r = x / (HD / 8), ch = x % (HD / 8);
-                    if (r >= from && r < to) continue;
-                    *reinterpret_cast<uint4*>(smem_raw + (vb - smem_u32(smem_raw)) + (ch >> 3) * S::kPanel + r * 128 + ((ch & 7) << 4)) = make_uint4(0, 0, 0, 0);
-                }
-                fence_proxy_async();
-                __syncwarp();
-            }
-#pragma unroll
-            for (uint32_t h = 0; h < 2 && ok; h++) {
-                wait(p_full + 16 * i + 8 * h, j & 1);
+        for (uint32_t n = 0; n < halves && ok; n++) {
+            const uint32_t j = n >> 1, h = n & 1, uv = 2 * j + 1, uk = 2 * j + 2, k0 = start + (b0 + j) * kKeys, vb = slot_of_use(uv);
+            const bool last = n + 1 == halves;
+            if (h == 0) {
+                wait_full(uv);
                 if (!ok) break;
-                if (elect_one()) {
-#pragma unroll
-                    for (int s = 4 * (int)h; s < 4 * (int)h + 4; s++)
-                        umma_f16_ts(o_cols, s_cols + 8 * s, desc_mn_sw128(vb + s * 2048, S::kPanel), idesc_of<T>(128, HD, 1), j > 0 || s > 0);
-                    if (h == 1) umma_commit(last ? done + 8 * i : empty + 8 * (uv % S::kSlots));
+                if (k0 < lo || k0 + kKeys > hi) {                // zeros where no row looks: the copies have left there what lay there, or the neighbours of what was asked for
+                    const uint32_t from = lo > k0 ? lo - k0 : 0, to = hi - k0;
+                    for (uint32_t x = lane; x < kKeys * (HD / 8); x += 32) {
+                        const uint32_t r = x / (HD / 8), ch = x % (HD / 8);
+                        if (r >= from && r < to) continue;
+                        *reinterpret_cast<uint4*>(smem_raw + (vb - smem_u32(smem_raw)) + (ch >> 3) * S::kPanel + r * 128 + ((ch & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
                 }
-                __syncwarp();
             }
+            wait(p_full + 16 * i + 8 * h, j & 1);
             if (!ok) break;
+            if (elect_one()) {
+#pragma unroll
+                for (int s = 0; s < 4; s++)
+                    umma_f16_ts(o_cols, s_cols + 64 * h + 8 * s, desc_mn_sw128(vb + (4 * h + s) * 2048, S::kPanel), idesc_of<T>(128, HD, 1), n > 0 || s > 0);
+                umma_commit(last ? done + 8 * i : o_full + 8 * i);
+                if (h && !last) umma_commit(empty + 8 * (uv % S::kSlots));
+            }
+            __syncwarp();
             if (last) {
                 n_d++;
                 break;
             }
-            wait_full(uk);
-            if (ok) scores(uk);
+            n_o++;
+            if (n + 2 < halves) {
+                if (h == 0) wait_full(uk);
+                if (ok) scores(uk, h);
+            }
         }
-        mbar_drain(s_full + 8 * i, 1, n_s);    // nor is a product when the tensor memory goes back
+        mbar_drain(s_full + 16 * i, 1, n_s[0]);                  // nor is a product when the tensor memory goes back
+        mbar_drain(s_full + 16 * i + 8, 1, n_s[1]);
+        mbar_drain(o_full + 8 * i, 1, n_o);
         mbar_drain(done + 8 * i, 1, n_d);
     } else {
         const uint32_t lanes = (warp & 3) << 21, s_cols = tmem + 128 * chain + lanes, o_cols = tmem + 256 + 128 * chain + lanes;
@@ -336,59 +335,53 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
         float ref = -INFINITY, l = 0.f;
         bool cut = false;                      // some block had positions that this row does not see
         if (chain < chains) {
-            for (uint32_t j = 0; j < n_blocks; j++) {
-                if (ok) ok = mbar_wait_timed(s_full + 8 * chain, j & 1, &abort_flag);
+            for (uint32_t n = 0; n < 2 * n_blocks; n++) {
+                const uint32_t h = n & 1, k0 = start + (b0 + (n >> 1)) * kKeys + 64 * h, cols = s_cols + 64 * h;
+                if (ok) ok = mbar_wait_timed(s_full + 16 * chain + 8 * h, (n >> 1) & 1, &abort_flag);
                 __syncwarp();
                 tc_fence_after_sync();
-                const uint32_t k0 = start + (b0 + j) * kKeys;
-                const bool inside = k0 >= row_lo && k0 + kKeys <= row_hi, easy = __all_sync(0xffffffffu, plain && inside && a.cap == 0.f);
+                const bool inside = k0 >= row_lo && k0 + 64 <= row_hi;
                 cut |= !inside;
-                // 32 scores, of which `mul` times are in units of log2
-                auto load = [&](uint32_t (&r)[32], uint32_t q) {
-                    tmem_ld32(s_cols + 32 * q, r);
-                    tmem_ld_wait();
-                    if (easy) return;
-                    if (a.cap != 0.f) tanh_scores(reinterpret_cast<float(&)[32]>(r), to_cap);
-                    if (a.slopes || !plain) {
-                        const float at_0 = -slope * (float)(pos - (int32_t)(k0 + 32 * q));
+                uint32_t r[2][32];
+                tmem_ld32(cols, r[0]);
+                tmem_ld32(cols + 32, r[1]);
+                tmem_ld_wait();
+                // scores, of which `mul` times are in units of log2
+                if (!__all_sync(0xffffffffu, plain && inside && a.cap == 0.f)) {
 #pragma unroll
-                        for (int e = 0; e < 32; e++) r[e] = __float_as_uint(fmaf(__uint_as_float(r[e]), pre, fmaf(slope, (float)e, at_0)));
+                    for (uint32_t q = 0; q < 2; q++) {
+                        if (a.cap != 0.f) tanh_scores(reinterpret_cast<float(&)[32]>(r[q]), to_cap);
+                        if (!plain) {
+                            const float at_0 = -slope * (float)(pos - (int32_t)(k0 + 32 * q));
+#pragma unroll
+                            for (int e = 0; e < 32; e++) r[q][e] = __float_as_uint(fmaf(__uint_as_float(r[q][e]), pre, fmaf(slope, (float)e, at_0)));
+                        }
                     }
                     if (!__all_sync(0xffffffffu, inside)) {
 #pragma unroll
-                        for (int e = 0; e < 32; e++) {
-                            const uint32_t key = k0 + 32 * q + e;
-                            if (key < row_lo || key >= row_hi) r[e] = 0xFF800000u;
-                        }
-                    }
-                };
-                auto most = [&](const uint32_t (&r)[32], float m0) {
-                    float m1 = -INFINITY;
+                        for (uint32_t q = 0; q < 2; q++)
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        m0 = max3(m0, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
-                        m1 = max3(m1, __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
+                            for (int e = 0; e < 32; e++) {
+                                const uint32_t key = k0 + 32 * q + e;
+                                if (key < row_lo || key >= row_hi) r[q][e] = 0xFF800000u;
+                            }
                     }
-                    return fmaxf(m0, m1);
-                };
-                uint32_t r0[32], r1[32], r2[32];
-                load(r0, 0);
-                float top = most(r0, -INFINITY);
-                load(r1, 1);
-                top = most(r1, top);
-#pragma unroll
-                for (uint32_t q = 2; q < 4; q++) {
-                    load(r2, q);
-                    top = most(r2, top);
-                    if (!easy) tmem_st32(s_cols + 32 * q, r2);   // these are read again below
                 }
-                top *= mul;
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int q = 0; q < 2; q++)
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(r[q][e]), __uint_as_float(r[q][e + 1]));
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
                 const bool rise = top > ref + kRise || (ref == -INFINITY && top > ref);
                 const float corr = rise ? exp2_approx(ref - top) : 1.f;
                 l *= corr;
                 ref = rise ? top : ref;
-                // S of this block comes behind the product of the last one: O is complete
-                if (__any_sync(0xffffffffu, rise) && j > 0) {
+                if (__any_sync(0xffffffffu, rise) && n > 0) {
+                    // O with the last half's product: the one before it is behind these scores, so one of two phases is on
+                    if (ok) ok = mbar_wait_timed(o_full + 8 * chain, (n - 1) & 1, &abort_flag);
+                    __syncwarp();
+                    tc_fence_after_sync();
 #pragma unroll 1
                     for (int q = 0; q < HD / 16; q++) {
                         uint32_t o[16];
@@ -402,38 +395,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
                 const float sub = ref == -INFINITY ? 0.f : ref;
                 const uint64_t mul2 = packf(mul), sub2 = packf(-sub);
                 uint64_t both = 0;
-                // 32 weights into 16 columns.  They meet the values in the cache's type: half a step of it, relative, each; their sum is that of the 32-bit ones.
-                auto weights = [&](const uint32_t (&r)[32], uint32_t q) {
+                // The weights meet the values in the cache's type: half a step of it, relative, each; their sum is that of the 32-bit ones.
+#pragma unroll
+                for (uint32_t q = 0; q < 2; q++) {
                     uint32_t p[16];
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
-                        const uint64_t x = ffma2(pack2(r[2 * e], r[2 * e + 1]), mul2, sub2);
+                        const uint64_t x = ffma2(pack2(r[q][2 * e], r[q][2 * e + 1]), mul2, sub2);
                         const float p0 = exp2_approx(__uint_as_float((uint32_t)x)), p1 = exp2_approx(__uint_as_float((uint32_t)(x >> 32)));
                         both = fadd2(both, pack2(__float_as_uint(p0), __float_as_uint(p1)));
                         p[e] = Half2<T>::pack(p0, p1);
                     }
-                    tmem_st16(s_cols + 16 * q, p);
-                };
-                auto hand_over = [&](uint32_t h) {
-                    tmem_st_wait();
-                    tc_fence_before_sync();
-                    mbar_arrive(p_full + 16 * chain + 8 * h);
-                };
-                // The tiles take their exponentials in turn (block j of the second one behind block j of the first, and that behind block j - 1 of the second): the
-                // products of one run under the exponentials of the other.  Left alone they fall into step, 4300 clocks a block instead of 3900.
-                if (ok && chains == 2 && (chain == 1 || j > 0)) ok = mbar_wait_timed(turn + 8 * chain, (chain == 1 ? j : j - 1) & 1, &abort_flag);
-                __syncwarp();
-                weights(r0, 0);
-                weights(r1, 1);
-                hand_over(0);
-#pragma unroll
-                for (uint32_t q = 2; q < 4; q++) {
-                    tmem_ld32(s_cols + 32 * q, r2);
-                    tmem_ld_wait();
-                    weights(r2, q);
+                    tmem_st16(cols + 16 * q, p);
                 }
-                if (lane == 0) mbar_arrive(turn + 8 * (chain ^ 1));
-                hand_over(1);
+                tmem_st_wait();
+                tc_fence_before_sync();
+                mbar_arrive(p_full + 16 * chain + 8 * h);
                 l += sum2(both);
             }
             if (n_blocks > 0 && ok) ok = mbar_wait_timed(done + 8 * chain, 0, &abort_flag);
