@@ -755,10 +755,8 @@ static int32_t encode(runit_ctx* ctx, const runit_paged_cfg* g, void* pages, CUt
 template <typename T, int HD>
 static int32_t run(runit_ctx* ctx, const runit_paged_cfg* g, const runit_paged_batch* b, const AttnArgs& a, const Choice& c, uint8_t* s, const Layout& l) {
     int32_t st;
-    const TcArgs pre{min(g->page, 128u), c.pre_split, true, false, (float*)(s + l.pre_part_o), (float*)(s + l.pre_part_ml)};
-    const TcArgs own{min(g->page, 128u), c.own_split, false, c.direct, (float*)(s + l.own_part_o), (float*)(s + l.own_part_ml)};
-    if (c.pre_tc && (st = paged_attention_tc(ctx, g, a, pre, c.pre_tiles)) != RUNIT_OK) return st;
-    if (c.own_tc && (st = paged_attention_tc(ctx, g, a, own, c.own_tiles)) != RUNIT_OK) return st;
+    TcArgs pre{min(g->page, 128u), c.pre_split, true, false, false, (float*)(s + l.pre_part_o), (float*)(s + l.pre_part_ml)};
+    TcArgs own{min(g->page, 128u), c.own_split, false, c.direct, false, (float*)(s + l.own_part_o), (float*)(s + l.own_part_ml)};
     uint32_t share = 0;
     if (c.n_entries) {
         constexpr uint32_t smem = Shape<HD>::kRing + 1024 + (kMaxSeqs + 2) * 4;
@@ -774,6 +772,12 @@ static int32_t run(runit_ctx* ctx, const runit_paged_cfg* g, const runit_paged_b
         if ((st = runit_after_launch(ctx, "paged_attention")) != RUNIT_OK) return st;
         share = grid * kWarps / max(1u, c.n_entries * g->kv_heads);
     }
+    // A launch behind another one of this call reads nothing of it, and takes the SMs that it leaves: 128 rows behind 32768 positions 120 -> 115 us.  Only the
+    // second one: its own successor could not rely on its having waited.
+    pre.beside = c.n_entries > 0;
+    own.beside = c.n_entries > 0 ? !c.pre_tc : c.pre_tc;
+    if (c.pre_tc && (st = paged_attention_tc(ctx, g, a, pre, c.pre_tiles)) != RUNIT_OK) return st;
+    if (c.own_tc && (st = paged_attention_tc(ctx, g, a, own, c.own_tiles)) != RUNIT_OK) return st;
     if (c.direct) return RUNIT_OK;
     const MergeArgs m{c.n_entries, c.own_tc ? c.own_split : 0, c.pre_tc ? c.pre_split : 0, own.part_o, own.part_ml, pre.part_o, pre.part_ml, b->shared_len != 0};
     // a block for each where a segment has more pieces than a warp asks for at once, when all are alike

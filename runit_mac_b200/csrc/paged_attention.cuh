@@ -28,6 +28,7 @@ struct AttnArgs {
 struct TcArgs {
     uint32_t box, split;     // positions of a copy; parts that a tile's positions are cut into
     bool shared, direct;     // direct: a row is done with this launch
+    bool beside;             // the launch in front belongs to the same call and has waited for what came before: nothing of it is read here
     float *part_o, *part_ml; // [split][rows * heads][dim] and [..][2]
 };
 int32_t paged_attention_tc(runit_ctx* ctx, const runit_paged_cfg* g, const AttnArgs& a, TcArgs w, uint32_t tiles);

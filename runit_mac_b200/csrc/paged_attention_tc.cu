@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = tmem_holder;
-    grid_dependency_wait();
+    if (!w.beside) grid_dependency_wait();
     grid_launch_dependents();
 
     // which rows and positions
@@ -495,6 +495,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
         tc_fence_after_sync();
         tmem_dealloc(tmem, 512);
     }
+    if (w.beside) grid_dependency_wait();      // whoever waits for this launch waits for the one in front, too
 }
 
 template <typename T, int HD>
