@@ -81,6 +81,11 @@ template <> struct Half2<__nv_bfloat16> {
 // the 16-bit halves of w that are no numbers, set to zero
 template <typename T> __device__ __forceinline__ uint32_t finite_part(uint32_t w, uint32_t nf) { return w & ~((nf >> 15) * 0xFFFFu); }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 // tanh(k v) of N products, for a whole warp.  Below 0.35 tanh u = u (1 - u^2/3 + 2 u^4/15 - 17 u^6/315 + 62 u^8/2835), its Taylor series, whose next
 // term is 2.4e-7 of u there; a warp with a larger argument takes (1 - e^-2|u|) / (1 + e^-2|u|), off by some 2^-22.
 template <int N> __device__ __forceinline__ void tanh_scores(float (&v)[N], float k) {
@@ -91,7 +96,7 @@ template <int N> __device__ __forceinline__ void tanh_scores(float (&v)[N], floa
     for (int i = 0; i < N / 2; i++) {
         u[i] = fmul2(pack2(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1])), k2);
         w[i] = fmul2(u[i], u[i]);
-        most = fmaxf(most, fmaxf(__uint_as_float((uint32_t)w[i]), __uint_as_float((uint32_t)(w[i] >> 32))));
+        most = max3(most, __uint_as_float((uint32_t)w[i]), __uint_as_float((uint32_t)(w[i] >> 32)));
     }
     if (__any_sync(0xffffffffu, most > 0.35f * 0.35f)) {
 #pragma unroll

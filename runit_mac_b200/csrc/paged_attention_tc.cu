@@ -31,11 +31,6 @@ template <typename T> __host__ __device__ constexpr uint32_t idesc_of(uint32_t m
 template <> __host__ __device__ constexpr uint32_t idesc_of<__half>(uint32_t m, uint32_t n, uint32_t b_mn) { return umma_idesc_f16(m, n, b_mn); }
 template <> __host__ __device__ constexpr uint32_t idesc_of<__nv_bfloat16>(uint32_t m, uint32_t n, uint32_t b_mn) { return umma_idesc_f16(m, n, b_mn) | (1u << 7) | (1u << 10); }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
 // One row's attention over positions lo .. hi of a table, by a warp with plain arithmetic: for rows whose products met a value that is no number at a
 // position that they do not see (0 x Inf).  Returns maximum (log2 units) and sum; o: HD / 32 of the dimensions per lane.
 template <typename T, int HD>
@@ -115,7 +110,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
             found[0] = c.n_seqs;
             found[1] = index;
         }
-    } else {                                   // tiles in front of a sequence; the last ones (those with the most positions) begin
+    } else if (c.n_seqs <= 32) {               // all sequences' last tiles first, then those in front of them: those with the most positions begin
+        if (warp == 0) {
+            const uint32_t n = lane < c.n_seqs ? (sequence(c, lane).n * c.group + kTcRows - 1) / kTcRows : 0;
+            if (index < __reduce_add_sync(0xffffffffu, n)) {
+                uint32_t r = 0;                // tiles of every sequence that come before the one that is looked for
+                for (uint32_t step = 1u << 23; step > 0; step /= 2)
+                    if (__reduce_add_sync(0xffffffffu, min(n, r + step)) <= index) r += step;
+                const uint32_t rest = index - __reduce_add_sync(0xffffffffu, min(n, r)), has = __ballot_sync(0xffffffffu, n > r);
+                uint32_t e = has;
+                for (uint32_t i = 0; i < rest; i++) e &= e - 1;
+                e = __ffs(e) - 1;
+                const uint32_t tiles = __shfl_sync(0xffffffffu, n, e);
+                if (lane == 0) {
+                    found[0] = e;
+                    found[1] = tiles - 1 - r;
+                }
+            }
+        }
+    } else {                                   // tiles in front of a sequence; the last ones begin
         const uint32_t per = (c.n_seqs + kTcThreads - 1) / kTcThreads, beg = min(c.n_seqs, tid * per), end = min(c.n_seqs, beg + per);
         uint32_t sum = 0;
         for (uint32_t e = beg; e < end; e++) sum += (sequence(c, e).n * c.group + kTcRows - 1) / kTcRows;
