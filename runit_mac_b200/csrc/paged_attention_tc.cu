@@ -69,14 +69,14 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const AttnArgs a, const TcArgs w) {
     using S = TcShape<HD>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * S::kSlots + 12];
+    __shared__ __align__(8) uint64_t bars[2 * S::kSlots + 14];
     __shared__ uint32_t tmem_holder, found[4], sums[kTcThreads / 32];
     __shared__ volatile int abort_flag;
     const Cache& c = a.c;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    // full, empty: one phase per use of a slot; s_full, p_full of a tile's halves: one per block; o_full: one per half block; done: one
-    const uint32_t full = smem_u32(bars), empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots, p_full = s_full + 32, o_full = p_full + 32, done = o_full + 16;
+    // full, empty: one phase per use of a slot; s_full, p_full of a tile's halves: one per block; o_full, turn: one per half block; done: one
+    const uint32_t full = smem_u32(bars), empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots, p_full = s_full + 32, o_full = p_full + 32, done = o_full + 16, turn = done + 16;
     if (tid == 0) {
         abort_flag = 0;
         found[0] = 0xFFFFFFFFu;
@@ -208,6 +208,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
         for (uint32_t i = 0; i < 2; i++) {
             mbar_init(o_full + 8 * i, 1);
             mbar_init(done + 8 * i, 1);
+            mbar_init(turn + 8 * i, 4);
         }
         for (uint32_t i = 0; i < 4; i++) {
             mbar_init(s_full + 8 * i, 1);
@@ -408,6 +409,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
                 const float sub = ref == -INFINITY ? 0.f : ref;
                 const uint64_t mul2 = packf(mul), sub2 = packf(-sub);
                 uint64_t both = 0;
+                // The tiles take their exponentials in turn (half n of the second one behind half n of the first, and that behind half n - 1 of the second).  Left
+                // alone they fall into step and do everything side by side (2900 clocks a half with a cap, 2500 in turn).
+                if (ok && chains == 2 && (chain == 1 || n > 0)) ok = mbar_wait_timed(turn + 8 * chain, (chain == 1 ? n : n - 1) & 1, &abort_flag);
+                __syncwarp();
                 // The weights meet the values in the cache's type: half a step of it, relative, each; their sum is that of the 32-bit ones.
 #pragma unroll
                 for (uint32_t q = 0; q < 2; q++) {
@@ -421,6 +426,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
                     }
                     tmem_st16(cols + 16 * q, p);
                 }
+                if (lane == 0) mbar_arrive(turn + 8 * (chain ^ 1));
                 tmem_st_wait();
                 tc_fence_before_sync();
                 mbar_arrive(p_full + 16 * chain + 8 * h);
