@@ -2,6 +2,8 @@
 //
 // With m = max x, d = x - m, Z = sum e^d: log p = d - log Z, entropy = log Z - (sum e^d d) / Z.  The maximal entry's own 1 is kept out of the sum, Z = 1 + z
 // and log Z = log1p(z): when that entry holds nearly all of the mass, its log probability and the entropy are tiny and keep their digits.
+// Bound: HBM and the issue slots, close to each other: 2048 rows of 152064 bf16 logits with 5 alternatives take 136 us, 4.6 TB/s.  Few rows: latency; 8 rows of
+// 151936 with 20 alternatives, a cluster of 16 blocks for each, 16.6 us.
 #include "gemv_common.cuh"
 #include "paged.cuh"
 #include "tcgen05.cuh"
@@ -244,7 +246,7 @@ template <typename T, bool TOP> struct Pass {
 #pragma unroll
         for (int j = 0; j < V; j++) below(u[j], most[j], i + 32 * j);
     }
-    // a vector below the maximum.  (Packed pairs are half the multiply-adds, on one of two pipes, and moves to form them: no gain.)
+    // a vector below the maximum
     __device__ __forceinline__ void below(const uint4& u, float most, uint32_t i) {
         if (TOP) note(most, i);
         float v[N];

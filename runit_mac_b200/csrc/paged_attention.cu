@@ -109,7 +109,7 @@ __device__ __noinline__ void add_not_finite(const uint8_t* stage_v, uint32_t k0,
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const AttnArgs a,
-                                                                   const uint32_t e0, const uint32_t n_entries) {
+                                                                   const uint32_t n_entries) {
     using S = Shape<HD>;
     constexpr uint32_t KS = HD / 16, ND = HD / 8, NK = kStep / 8;
     extern __shared__ uint8_t smem_raw[];
@@ -119,6 +119,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
     uint32_t* const before = reinterpret_cast<uint32_t*>(ring + S::kRing);         // [n_entries + 1] steps in front of an entry
     const Cache& c = a.c;
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g4 = lane >> 2, t4 = lane & 3;
+    if (tid == 0) {
+        prefetch_map(&mk);
+        prefetch_map(&mv);
+    }
     if (tid < kWarps * S::kStages) mbar_init(smem_u32(&bars[tid]), 1);
     if (tid == 0) {
         edge[0] = c.shared;
@@ -142,7 +146,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
         pre_hi = max(pre_hi, min(s.len, c.shared));
     };
     auto cost = [&](uint32_t e) {
-        const Entry t = entry_of(a, e0 + e, pre_lo, pre_hi);
+        const Entry t = entry_of(a, e, pre_lo, pre_hi);
         return t.tiles * t.steps * c.kv_heads;
     };
     auto scan = [&](uint32_t v) {
@@ -153,7 +157,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
         }
         return v;
     };
-    const bool with_pre = e0 + n_entries > c.n_seqs;
+    const bool with_pre = n_entries > c.n_seqs;
     if (n_entries <= kFew) {
         if (with_pre) {
             for (uint32_t e = lane; e < c.n_seqs; e += 32) seen(e);
@@ -217,8 +221,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
         a.plan[0] = pre_lo;
         a.plan[1] = pre_hi;
         a.plan[2] = workers;
-        a.plan[3] = e0;
-        a.plan[4] = total;
+        a.plan[3] = total;
     }
     if (x0 == x1) return;
 
@@ -246,7 +249,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
                 u.h = 0;
                 if (x >= total) return;
                 uint32_t some = 0;             // the next entry that has steps (there is one)
-                for (u.e++; !(some = __ballot_sync(0xffffffffu, u.e - e0 + lane < n_entries && cost(u.e - e0 + lane))) && u.e - e0 < n_entries; u.e += 32) {}
+                for (u.e++; !(some = __ballot_sync(0xffffffffu, u.e + lane < n_entries && cost(u.e + lane))) && u.e < n_entries; u.e += 32) {}
                 u.e += __ffs(some) - 1;
                 u.t = entry_of(a, u.e, pre_lo, pre_hi);
             }
@@ -258,7 +261,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
 
     const uint32_t bar0 = smem_u32(&bars[warp * S::kStages]), ring0 = smem_u32(ring) + warp * S::kStages * S::kStage;
     Cursor in, at;
-    at.e = e0 + e_first;
+    at.e = e_first;
     at.t = entry_of(a, at.e, pre_lo, pre_hi);
     {
         const uint32_t of = x0 - e_before, seg = of / at.t.steps;
@@ -539,7 +542,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
 // Adds up what the launches have left of a (row, query head): a warp for each, or a block (WIDE) where a segment has many pieces.  A lane has the maximum and sum
 // of a piece, the factors 2^(m - max m) go round, and every lane adds up 2 or 4 of the dimensions.  Rows that a worker has written itself are left.
 struct MergeArgs {
-    uint32_t n_entries;                        // of the split kernel: 0 when it has not run
+    uint32_t n_entries;                        // of the split kernel: 0 when it has not run (all sequences, and the shared positions if their rows are few)
     uint32_t own_parts, pre_parts;             // parts of the kernel for many rows: 0 when the split kernel has had those positions
     const float *own_o, *own_ml, *pre_o, *pre_ml;
     bool shared;
@@ -563,16 +566,16 @@ __device__ __forceinline__ uint32_t sequence_by_warp(const Cache& c, uint32_t ro
 template <typename T, int HD, bool WIDE>
 __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttnArgs a, const MergeArgs g) {
     constexpr uint32_t E = HD / 32;
-    grid_dependency_wait();
-    grid_launch_dependents();
     const Cache& c = a.c;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint64_t pairs = (uint64_t)c.rows * c.heads, orow = WIDE ? blockIdx.x : (uint64_t)blockIdx.x * kMergeWarps + warp;
-    if (orow >= pairs) return;
+    // What came before the launches of this call was over before any of them began: the lengths are read ahead of the wait, which every warp does all the same, as
+    // whoever comes next relies on this launch's being the last to end.
     const uint32_t token = (uint32_t)(orow / c.heads), head = (uint32_t)(orow % c.heads);
-    const uint32_t s = sequence_by_warp(c, token);
-    if (s >= c.n_seqs) return;
-    const Seq q = sequence(c, s);
+    const uint32_t s = orow < pairs ? sequence_by_warp(c, token) : c.n_seqs;
+    const Seq q = s < c.n_seqs ? sequence(c, s) : Seq{0, 0, 0};
+    grid_dependency_wait();
+    grid_launch_dependents();
     if (token < q.row0 || token >= q.row0 + q.n) return;
     // pieces of one entry: as many, from worker w0 on, or one that is whole
     struct List {
@@ -589,14 +592,12 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttnArgs 
     };
     List own{g.own_parts, 0, 0, 0}, pre{g.pre_parts, 0, 0, 0};
     if (g.n_entries) {
-        const uint32_t pre_lo = a.plan[0], pre_hi = a.plan[1], e0 = a.plan[3];
+        const uint32_t pre_lo = a.plan[0], pre_hi = a.plan[1];
         workers = a.plan[2];
-        total = a.plan[4];
-        if (!g.own_parts) {
-            own = list_of(entry_of(a, s, pre_lo, pre_hi), s - e0, (token - q.row0) * c.group + head % c.group);
-            if (own.n == 1 && !g.shared) return;
-        }
-        if (g.shared && !g.pre_parts) pre = list_of(entry_of(a, c.n_seqs, pre_lo, pre_hi), c.n_seqs - e0, token * c.group + head % c.group);
+        total = a.plan[3];
+        own = list_of(entry_of(a, s, pre_lo, pre_hi), s, (token - q.row0) * c.group + head % c.group);
+        if (own.n == 1 && !g.shared) return;
+        if (g.shared && !g.pre_parts) pre = list_of(entry_of(a, c.n_seqs, pre_lo, pre_hi), c.n_seqs, token * c.group + head % c.group);
     }
     const uint32_t n = own.n + pre.n, step = WIDE ? kMergeWarps : 1;
     float m = -INFINITY, l = 0.f, o[E];
@@ -622,6 +623,22 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttnArgs 
                 pml = y.ml + x.row * 2;
             }
         }
+        // the sums of the first eight are asked for along with the maxima
+        const uint64_t at = reinterpret_cast<uint64_t>(po);
+        float v[8][E];
+        auto ask = [&](uint32_t k, float (&x)[E]) {
+            const float* y = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, at, k & 31));
+            if (k >= count) return;
+            if constexpr (E == 4) {
+                const float4 z = *reinterpret_cast<const float4*>(y + 4 * lane);
+                x[0] = z.x; x[1] = z.y; x[2] = z.z; x[3] = z.w;
+            } else {
+                const float2 z = *reinterpret_cast<const float2*>(y + 2 * lane);
+                x[0] = z.x; x[1] = z.y;
+            }
+        };
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++) ask(k, v[k]);
         const float2 ml = pml ? *reinterpret_cast<const float2*>(pml) : make_float2(-INFINITY, 0.f);
         float top = fmaxf(m, ml.x);
 #pragma unroll
@@ -635,18 +652,17 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttnArgs 
         m = top;
 #pragma unroll
         for (uint32_t e = 0; e < E; e++) o[e] *= old;
-        const uint64_t at = reinterpret_cast<uint64_t>(po);
-#pragma unroll 8
-        for (uint32_t k = 0; k < count; k++) {
-            const float* x = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, at, k));
-            const float fk = __shfl_sync(0xffffffffu, f, k);
-            if constexpr (E == 4) {
-                const float4 v = *reinterpret_cast<const float4*>(x + 4 * lane);
-                o[0] = fmaf(fk, v.x, o[0]); o[1] = fmaf(fk, v.y, o[1]); o[2] = fmaf(fk, v.z, o[2]); o[3] = fmaf(fk, v.w, o[3]);
-            } else {
-                const float2 v = *reinterpret_cast<const float2*>(x + 2 * lane);
-                o[0] = fmaf(fk, v.x, o[0]); o[1] = fmaf(fk, v.y, o[1]);
+        for (uint32_t k0 = 0; k0 < count; k0 += 8) {
+#pragma unroll
+            for (uint32_t k = 0; k < 8; k++) {
+                const float fk = __shfl_sync(0xffffffffu, f, (k0 + k) & 31);
+                if (k0 + k >= count) continue;
+#pragma unroll
+                for (uint32_t e = 0; e < E; e++) o[e] = fmaf(fk, v[k][e], o[e]);
             }
+            if (k0 + 8 < count)
+#pragma unroll
+                for (uint32_t k = 0; k < 8; k++) ask(k0 + 8 + k, v[k]);
         }
     }
     if constexpr (WIDE) {
@@ -681,7 +697,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttnArgs 
 // 16.  The parts of the kernel for many rows: as many as fill 148 SMs best, of four blocks at least.
 struct Choice {
     bool own_tc, pre_tc, direct;
-    uint32_t own_tiles, pre_tiles, own_split, pre_split, e0, n_entries;
+    uint32_t own_tiles, pre_tiles, own_split, pre_split, n_entries;
 };
 static uint32_t parts_of(uint64_t ctas, uint64_t blocks) {
     uint32_t best = 1;
@@ -707,9 +723,7 @@ static Choice choose(const runit_paged_cfg* g, const runit_paged_batch* b) {
     c.own_split = parts_of((pairs / 256 + (b->n_seqs + 1) / 2) * g->kv_heads, (uint64_t)b->table_ld * g->page / 128);
     c.pre_split = parts_of((uint64_t)c.pre_tiles * g->kv_heads, b->shared_len / 128);
     c.direct = c.own_tc && !b->shared_len && c.own_split == 1;
-    const bool pre_split_kernel = b->shared_len && !c.pre_tc;
-    c.e0 = c.own_tc ? b->n_seqs : 0;
-    c.n_entries = (c.own_tc ? 0 : b->n_seqs) + (pre_split_kernel ? 1 : 0);
+    c.n_entries = c.own_tc ? 0 : b->n_seqs + (b->shared_len && !c.pre_tc ? 1 : 0);       // (own_tc: more than 32 pairs, so pre_tc as well)
     return c;
 }
 struct Layout {
@@ -768,14 +782,14 @@ static int32_t run(runit_ctx* ctx, const runit_paged_cfg* g, const runit_paged_b
         CUtensorMap mk, mv;
         if ((st = encode(ctx, g, g->k_pages, &mk)) != RUNIT_OK || (st = encode(ctx, g, g->v_pages, &mv)) != RUNIT_OK) return st;
         const uint32_t grid = min((uint32_t)ctx->sm_count, kMaxWorkers / kWarps);
-        runit_launch_chain_smem(ctx, paged_split_kernel<T, HD>, dim3(grid), dim3(kWarps * 32), smem, mk, mv, a, c.e0, c.n_entries);
+        runit_launch_chain_smem(ctx, paged_split_kernel<T, HD>, dim3(grid), dim3(kWarps * 32), smem, mk, mv, a, c.n_entries);
         if ((st = runit_after_launch(ctx, "paged_attention")) != RUNIT_OK) return st;
         share = grid * kWarps / max(1u, c.n_entries * g->kv_heads);
     }
     // A launch behind another one of this call reads nothing of it, and takes the SMs that it leaves: 128 rows behind 32768 positions 120 -> 115 us.  Only the
     // second one: its own successor could not rely on its having waited.
     pre.beside = c.n_entries > 0;
-    own.beside = c.n_entries > 0 ? !c.pre_tc : c.pre_tc;
+    own.beside = c.pre_tc;                     // the split kernel has not run
     if (c.pre_tc && (st = paged_attention_tc(ctx, g, a, pre, c.pre_tiles)) != RUNIT_OK) return st;
     if (c.own_tc && (st = paged_attention_tc(ctx, g, a, own, c.own_tiles)) != RUNIT_OK) return st;
     if (c.direct) return RUNIT_OK;

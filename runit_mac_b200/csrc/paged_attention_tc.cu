@@ -78,6 +78,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
     // full, empty: one phase per use of a slot; s_full, p_full of a tile's halves: one per block; o_full, turn: one per half block; done: one
     const uint32_t full = smem_u32(bars), empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots, p_full = s_full + 32, o_full = p_full + 32, done = o_full + 16, turn = done + 16;
     if (tid == 0) {
+        prefetch_map(&mk);
+        prefetch_map(&mv);
         abort_flag = 0;
         found[0] = 0xFFFFFFFFu;
         found[2] = c.shared;
