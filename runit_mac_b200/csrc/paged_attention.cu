@@ -16,6 +16,9 @@ constexpr uint32_t kWarps = 4, kStep = 32, kBox = 16, kRows = 16, kPlanHead = 16
 constexpr uint32_t kMaxWorkers = kWarps * 256;
 constexpr uint32_t kStepsMin = 2;              // a worker's share at least: what it costs to begin and to merge is that of about two steps
 constexpr uint32_t kFew = 256;                 // up to so many entries every warp finds its place for itself, without meeting the others
+// Up to so many, merge_kernel works out the plan for itself while the split kernel runs; else it is left in the scratch (64 sequences 47.7 -> 46.5 us; 128
+// behind shared positions, 3584 rows, 104.6 without and 105.3 with: too many warps, on SMs that are at work).
+constexpr uint32_t kFewMerged = 64;
 
 template <int HD> struct Shape {
     static constexpr uint32_t kBoxBytes = kBox * HD * 2, kStage = 4 * kBoxBytes, kStages = HD == 128 ? 3 : 6;
@@ -54,6 +57,19 @@ __device__ __forceinline__ Entry entry_of(const AttnArgs& a, uint32_t e, uint32_
     t.tiles = (t.n * c.group + kRows - 1) / kRows;
     t.steps = steps_of(t.lo, t.hi);
     return t;
+}
+__device__ __forceinline__ uint32_t cost_of(const AttnArgs& a, uint32_t e, uint32_t pre_lo, uint32_t pre_hi) {
+    const Entry t = entry_of(a, e, pre_lo, pre_hi);
+    return t.tiles * t.steps * a.c.kv_heads;
+}
+// The shared positions that some row of sequences e, e + step, ... sees.
+__device__ __forceinline__ void seen_of(const AttnArgs& a, uint32_t e, uint32_t step, uint32_t& lo, uint32_t& hi) {
+    for (; e < a.c.n_seqs; e += step) {
+        const Seq s = sequence(a.c, e);
+        if (!s.n) continue;
+        lo = min(lo, first_seen((int32_t)s.len - (int32_t)s.n, a.window));
+        hi = max(hi, min(s.len, a.c.shared));
+    }
 }
 // Worker w of `workers` has the steps from begin_of(w) to begin_of(w + 1): the first ones have one more than the others.
 __device__ __forceinline__ uint32_t begin_of(uint32_t w, uint32_t total, uint32_t workers) { return w * (total / workers) + min(w, total % workers); }
@@ -139,16 +155,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
         x0 = me < workers && total ? begin_of(me, total, workers) : 0;
         x1 = me < workers && total ? begin_of(me + 1, total, workers) : 0;
     };
-    auto seen = [&](uint32_t e) {              // the shared positions that some row of a sequence sees
-        const Seq s = sequence(c, e);
-        if (!s.n) return;
-        pre_lo = min(pre_lo, first_seen((int32_t)s.len - (int32_t)s.n, a.window));
-        pre_hi = max(pre_hi, min(s.len, c.shared));
-    };
-    auto cost = [&](uint32_t e) {
-        const Entry t = entry_of(a, e, pre_lo, pre_hi);
-        return t.tiles * t.steps * c.kv_heads;
-    };
+    auto cost = [&](uint32_t e) { return cost_of(a, e, pre_lo, pre_hi); };
     auto scan = [&](uint32_t v) {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -160,19 +167,24 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
     const bool with_pre = n_entries > c.n_seqs;
     if (n_entries <= kFew) {
         if (with_pre) {
-            for (uint32_t e = lane; e < c.n_seqs; e += 32) seen(e);
+            seen_of(a, lane, 32, pre_lo, pre_hi);
             pre_lo = __reduce_min_sync(0xffffffffu, pre_lo);
             pre_hi = __reduce_max_sync(0xffffffffu, pre_hi);
         }
         // (not unrolled: what a warp runs once costs most where its instructions come from)
+        uint32_t v = 0;
 #pragma unroll 1
-        for (uint32_t k = 0; k < n_entries; k += 32) total += __reduce_add_sync(0xffffffffu, k + lane < n_entries ? cost(k + lane) : 0);
+        for (uint32_t k = 0; k < n_entries; k += 32) {
+            v = k + lane < n_entries ? cost(k + lane) : 0;
+            total += __reduce_add_sync(0xffffffffu, v);
+        }
         share();
         uint32_t at = 0;
 #pragma unroll 1
         for (uint32_t k = 0; k < n_entries; k += 32) {
-            const uint32_t v = k + lane < n_entries ? cost(k + lane) : 0, inc = scan(v) + at;
-            if (blockIdx.x == 0 && warp == 0 && k + lane < n_entries) a.plan[kPlanHead + k + lane] = inc - v;
+            if (n_entries > 32) v = k + lane < n_entries ? cost(k + lane) : 0;
+            const uint32_t inc = scan(v) + at;
+            if (n_entries > kFewMerged && blockIdx.x == 0 && warp == 0 && k + lane < n_entries) a.plan[kPlanHead + k + lane] = inc - v;
             const uint32_t here = __ballot_sync(0xffffffffu, v && x0 >= inc - v && x0 < inc);
             if (here) {
                 e_first = k + __ffs(here) - 1;
@@ -182,7 +194,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
         }
     } else {
         if (with_pre) {
-            for (uint32_t e = tid; e < c.n_seqs; e += kWarps * 32) seen(e);
+            seen_of(a, tid, kWarps * 32, pre_lo, pre_hi);
             atomicMin(&edge[0], pre_lo);
             atomicMax(&edge[1], pre_hi);
             __syncthreads();
@@ -217,11 +229,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
         e_first = l;
         e_before = before[l];
     }
-    if (blockIdx.x == 0 && tid == 0) {
+    if (n_entries > kFewMerged && blockIdx.x == 0 && tid == 0) {
         a.plan[0] = pre_lo;
         a.plan[1] = pre_hi;
-        a.plan[2] = workers;
-        a.plan[3] = total;
+        a.plan[2] = total;
+        a.plan[3] = workers;
     }
     if (x0 == x1) return;
 
@@ -387,12 +399,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
 
     bool ok = true;
     uint32_t begun = x0 - at.step;             // where the segment begins in the order of steps
-    begin();
     for (uint32_t s = 0; s < S::kStages && xin < x1; s++) {
         copy(s);
         xin++;
         if (xin < x1) advance(xin);
     }
+    begin();
     for (uint32_t x = x0; x < x1 && ok; x++) {
         const uint32_t n = x - x0, stage = n % S::kStages;
         ok = __all_sync(0xffffffffu, mbar_wait(bar0 + 8 * stage, (n / S::kStages) & 1));
@@ -542,7 +554,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
 // Adds up what the launches have left of a (row, query head): a warp for each, or a block (WIDE) where a segment has many pieces.  A lane has the maximum and sum
 // of a piece, the factors 2^(m - max m) go round, and every lane adds up 2 or 4 of the dimensions.  Rows that a worker has written itself are left.
 struct MergeArgs {
-    uint32_t n_entries;                        // of the split kernel: 0 when it has not run (all sequences, and the shared positions if their rows are few)
+    uint32_t n_entries, most;                  // of the split kernel, and its workers at most: no entries when it has not run (all sequences, and the shared positions if their rows are few)
     uint32_t own_parts, pre_parts;             // parts of the kernel for many rows: 0 when the split kernel has had those positions
     const float *own_o, *own_ml, *pre_o, *pre_ml;
     bool shared;
@@ -574,6 +586,26 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttnArgs 
     const uint32_t token = (uint32_t)(orow / c.heads), head = (uint32_t)(orow % c.heads);
     const uint32_t s = orow < pairs ? sequence_by_warp(c, token) : c.n_seqs;
     const Seq q = s < c.n_seqs ? sequence(c, s) : Seq{0, 0, 0};
+    // the split kernel's plan, as far as it concerns this row; that of many entries it has left in the scratch
+    uint32_t workers = 1, total = 0, pre_lo = c.shared, pre_hi = 0, before = 0, before_pre = 0;
+    if (g.n_entries && g.n_entries <= kFewMerged) {
+        if (g.n_entries > c.n_seqs) {
+            seen_of(a, lane, 32, pre_lo, pre_hi);
+            pre_lo = __reduce_min_sync(0xffffffffu, pre_lo);
+            pre_hi = __reduce_max_sync(0xffffffffu, pre_hi);
+        }
+#pragma unroll 1
+        for (uint32_t k = lane; k < g.n_entries; k += 32) {
+            const uint32_t v = cost_of(a, k, pre_lo, pre_hi);
+            total += v;
+            if (k < s) before += v;
+            if (k < c.n_seqs) before_pre += v;
+        }
+        total = __reduce_add_sync(0xffffffffu, total);
+        before = __reduce_add_sync(0xffffffffu, before);
+        before_pre = __reduce_add_sync(0xffffffffu, before_pre);
+        workers = workers_of(total, g.most);
+    }
     grid_dependency_wait();
     grid_launch_dependents();
     if (token < q.row0 || token >= q.row0 + q.n) return;
@@ -581,23 +613,27 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttnArgs 
     struct List {
         uint32_t n, w0, beg, row;
     };
-    uint32_t workers = 1, total = 0;
-    auto list_of = [&](const Entry& u, uint32_t e, uint32_t i) {
+    auto list_of = [&](const Entry& u, uint32_t first, uint32_t i) {
         List x{0, 0, 0, i % kRows};
         if (u.steps == 0) return x;
-        x.beg = a.plan[kPlanHead + e] + (head / c.group * u.tiles + i / kRows) * u.steps;
+        x.beg = first + (head / c.group * u.tiles + i / kRows) * u.steps;
         x.w0 = owner_of(x.beg, total, workers);
         x.n = owner_of(x.beg + u.steps - 1, total, workers) - x.w0 + 1;
         return x;
     };
     List own{g.own_parts, 0, 0, 0}, pre{g.pre_parts, 0, 0, 0};
     if (g.n_entries) {
-        const uint32_t pre_lo = a.plan[0], pre_hi = a.plan[1];
-        workers = a.plan[2];
-        total = a.plan[3];
-        own = list_of(entry_of(a, s, pre_lo, pre_hi), s, (token - q.row0) * c.group + head % c.group);
+        if (g.n_entries > kFewMerged) {
+            pre_lo = a.plan[0];
+            pre_hi = a.plan[1];
+            total = a.plan[2];
+            workers = a.plan[3];
+            before = a.plan[kPlanHead + s];
+            if (g.n_entries > c.n_seqs) before_pre = a.plan[kPlanHead + c.n_seqs];
+        }
+        own = list_of(entry_of(a, s, pre_lo, pre_hi), before, (token - q.row0) * c.group + head % c.group);
         if (own.n == 1 && !g.shared) return;
-        if (g.shared && !g.pre_parts) pre = list_of(entry_of(a, c.n_seqs, pre_lo, pre_hi), c.n_seqs, token * c.group + head % c.group);
+        if (g.n_entries > c.n_seqs) pre = list_of(entry_of(a, c.n_seqs, pre_lo, pre_hi), before_pre, token * c.group + head % c.group);
     }
     const uint32_t n = own.n + pre.n, step = WIDE ? kMergeWarps : 1;
     float m = -INFINITY, l = 0.f, o[E];
@@ -771,7 +807,7 @@ static int32_t run(runit_ctx* ctx, const runit_paged_cfg* g, const runit_paged_b
     int32_t st;
     TcArgs pre{min(g->page, 128u), c.pre_split, true, false, false, (float*)(s + l.pre_part_o), (float*)(s + l.pre_part_ml)};
     TcArgs own{min(g->page, 128u), c.own_split, false, c.direct, false, (float*)(s + l.own_part_o), (float*)(s + l.own_part_ml)};
-    uint32_t share = 0;
+    uint32_t share = 0, most = 0;
     if (c.n_entries) {
         constexpr uint32_t smem = Shape<HD>::kRing + 1024 + (kMaxSeqs + 2) * 4;
         static bool configured[64] = {false};
@@ -784,7 +820,8 @@ static int32_t run(runit_ctx* ctx, const runit_paged_cfg* g, const runit_paged_b
         const uint32_t grid = min((uint32_t)ctx->sm_count, kMaxWorkers / kWarps);
         runit_launch_chain_smem(ctx, paged_split_kernel<T, HD>, dim3(grid), dim3(kWarps * 32), smem, mk, mv, a, c.n_entries);
         if ((st = runit_after_launch(ctx, "paged_attention")) != RUNIT_OK) return st;
-        share = grid * kWarps / max(1u, c.n_entries * g->kv_heads);
+        most = grid * kWarps;
+        share = most / (c.n_entries * g->kv_heads);
     }
     // A launch behind another one of this call reads nothing of it, and takes the SMs that it leaves: 128 rows behind 32768 positions 120 -> 115 us.  Only the
     // second one: its own successor could not rely on its having waited.
@@ -793,7 +830,7 @@ static int32_t run(runit_ctx* ctx, const runit_paged_cfg* g, const runit_paged_b
     if (c.pre_tc && (st = paged_attention_tc(ctx, g, a, pre, c.pre_tiles)) != RUNIT_OK) return st;
     if (c.own_tc && (st = paged_attention_tc(ctx, g, a, own, c.own_tiles)) != RUNIT_OK) return st;
     if (c.direct) return RUNIT_OK;
-    const MergeArgs m{c.n_entries, c.own_tc ? c.own_split : 0, c.pre_tc ? c.pre_split : 0, own.part_o, own.part_ml, pre.part_o, pre.part_ml, b->shared_len != 0};
+    const MergeArgs m{c.n_entries, most, c.own_tc ? c.own_split : 0, c.pre_tc ? c.pre_split : 0, own.part_o, own.part_ml, pre.part_o, pre.part_ml, b->shared_len != 0};
     // a block for each where a segment has more pieces than a warp asks for at once, when all are alike
     const uint64_t pairs = (uint64_t)g->heads * b->rows;
     if (share >= 16) runit_launch_chain(ctx, merge_kernel<T, HD, true>, dim3((uint32_t)pairs), dim3(kMergeWarps * 32), a, m);
