@@ -2,8 +2,8 @@
 //
 // With m = max x, d = x - m, Z = sum e^d: log p = d - log Z, entropy = log Z - (sum e^d d) / Z.  The maximal entry's own 1 is kept out of the sum, Z = 1 + z
 // and log Z = log1p(z): when that entry holds nearly all of the mass, its log probability and the entropy are tiny and keep their digits.
-// Bound: HBM and the issue slots, close to each other: 2048 rows of 152064 bf16 logits with 5 alternatives take 136 us, 4.6 TB/s.  Few rows: latency; 8 rows of
-// 151936 with 20 alternatives, a cluster of 16 blocks for each, 16.6 us.
+// Bound: HBM and the issue slots, close to each other: 2048 rows of 152064 bf16 logits with 5 alternatives take 122 us, 5.1 TB/s.  Few rows: latency; 8 rows of
+// 151936 with 20 alternatives, a cluster of 16 blocks for each, 13.0 us.
 #include "gemv_common.cuh"
 #include "paged.cuh"
 #include "tcgen05.cuh"
@@ -79,16 +79,25 @@ __device__ __forceinline__ void insert(Top& t, uint32_t v, uint32_t i) {
     if (lane == at) { t.v = v; t.i = i; }
     else if (lane > at) { t.v = uv; t.i = ui; }
 }
-// The first 32 of two such lists: the larger of one and the other from its end is a list that rises and falls, which five exchanges put in order.
-__device__ __forceinline__ void join(Top& t, const Top& o) {
+// The k largest entries of those that the lanes have at key(0) (a lane's next one comes up when next() is called in it), in descending order over the lanes.
+template <typename Key, typename Next> __device__ __forceinline__ Top largest(uint32_t k, Key key, Next next) {
     const uint32_t lane = threadIdx.x & 31;
-    const uint32_t ov = __shfl_sync(0xffffffffu, o.v, 31 - lane), oi = __shfl_sync(0xffffffffu, o.i, 31 - lane);
-    if (!before(t, ov, oi)) { t.v = ov; t.i = oi; }
-#pragma unroll
-    for (uint32_t d = 16; d > 0; d >>= 1) {
-        const uint32_t xv = __shfl_xor_sync(0xffffffffu, t.v, d), xi = __shfl_xor_sync(0xffffffffu, t.i, d);
-        if (before(t, xv, xi) == ((lane & d) != 0)) { t.v = xv; t.i = xi; }
+    Top t = {0, 0};
+#pragma unroll 1
+    for (uint32_t j = 0; j < k; j++) {
+        const Top mine = key();
+        const uint32_t v = __reduce_max_sync(0xffffffffu, mine.v);
+        if (v == 0) break;
+        uint32_t who = __ballot_sync(0xffffffffu, mine.v == v);
+        if (who & (who - 1)) {                 // equal ones: the lowest index
+            const uint32_t i = __reduce_max_sync(0xffffffffu, mine.v == v ? mine.i : 0);
+            who = __ballot_sync(0xffffffffu, mine.v == v && mine.i == i);
+        }
+        const uint32_t from = __ffs(who) - 1, i = __shfl_sync(0xffffffffu, mine.i, from);
+        if (lane == j) { t.v = v; t.i = i; }
+        if (lane == from) next();
     }
+    return t;
 }
 
 constexpr float kFloor = -1e38f;               // -Inf in the fast path, where the maximum is within kFar: far above the floor, and R is rounded by less than 2^-7
@@ -322,17 +331,30 @@ template <typename T, bool TOP> struct Pass {
     }
 };
 
-// Descending order of the lanes' entries.
-__device__ __forceinline__ void sort_lanes(Top& t) {
+// The first k of the warps' lists, in descending order.
+__device__ __forceinline__ Top first_of(const Top (&lists)[kWarps][32], uint32_t k) {
     const uint32_t lane = threadIdx.x & 31;
+    Top x[kWarps];
 #pragma unroll
-    for (uint32_t n = 2; n <= 32; n *= 2)
+    for (uint32_t w = 0; w < kWarps; w++) x[w] = lists[w][lane];
+    auto order2 = [&](uint32_t i, uint32_t j) {
+        if (before(x[i], x[j].v, x[j].i)) return;
+        const Top y = x[i];
+        x[i] = x[j];
+        x[j] = y;
+    };
+    // a lane's seven, by a network of sixteen exchanges
+    order2(0, 6); order2(2, 3); order2(4, 5);
+    order2(0, 2); order2(1, 4); order2(3, 6);
+    order2(0, 1); order2(2, 5); order2(3, 4);
+    order2(1, 2); order2(4, 6);
+    order2(2, 3); order2(4, 5);
+    order2(1, 2); order2(3, 4); order2(5, 6);
+    return largest(k, [&]() { return x[0]; }, [&]() {
 #pragma unroll
-        for (uint32_t d = n / 2; d > 0; d /= 2) {
-            const uint32_t xv = __shfl_xor_sync(0xffffffffu, t.v, d), xi = __shfl_xor_sync(0xffffffffu, t.i, d);
-            const bool up = (lane & n) != 0;                     // this stretch ascends
-            if (before(t, xv, xi) == (((lane & d) != 0) != up) && (t.v != xv || t.i != xi)) { t.v = xv; t.i = xi; }
-        }
+        for (uint32_t w = 0; w + 1 < kWarps; w++) x[w] = x[w + 1];
+        x[kWarps - 1] = Top{0, 0};
+    });
 }
 
 // Counted on mbarriers, with the suspension of mbar_try: a warp that polls takes issue slots from those that have data.
@@ -350,13 +372,14 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
     constexpr uint32_t N = Vec<T>::N;
     extern __shared__ __align__(128) uint8_t ring[];             // [kWarps][kStages][kStageBytes]
     __shared__ __align__(8) uint64_t bars[kWarps * kStages + 4];
-    __shared__ Sums part[2][kWarps], all;
-    __shared__ Top lists[2][kWarps][32], best[32];
+    __shared__ Sums part[2][kWarps], blocks[16];
+    __shared__ Top lists[2][kWarps][32], best[16][32];           // blocks, best: of a cluster, in its first block
     __shared__ uint32_t seconds[2][kWarps][32];
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, rank = blockIdx.x % cluster;
     if (tid < kWarps * kStages + 4) mbar_init(smem_u32(&bars[tid]), tid >= kWarps * kStages && tid < kWarps * kStages + 2 ? kWarps : 1);
     fence_mbar_init();
-    __syncthreads();
+    if (cluster > 1) cluster_sync();           // the others run, too: their shared memory can be written
+    else __syncthreads();
     grid_dependency_wait();
     grid_launch_dependents();
     const uint32_t there = smem_u32(&bars[kWarps * kStages]), taken = there + 16;          // of the two buffers that hold a row's findings
@@ -449,9 +472,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
             if (lane == 0) part[half][warp] = sums;
             if constexpr (TOP) {
                 seconds[half][warp][lane] = pass.others();
-                Top top = pass.top(w0 + lane, w1);
-                sort_lanes(top);
-                lists[half][warp][lane] = top;
+                lists[half][warp][lane] = pass.top(w0 + lane, w1);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(there + 8 * half);
@@ -460,18 +481,22 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
         }
         if (!ok) mbar_drain(bar0, kStages, asked);               // nothing is in flight when the block leaves
     }
+    bool listed = false;                       // the row's token is one of its entries, with the logit `given`
+    float given = 0.f;
+    auto token_of = [&](uint32_t row) {        // fetched ahead of the row's sums
+        if (lane > 0 || !a.tokens) return;
+        const int32_t token = a.tokens[row];
+        listed = (uint32_t)token < a.n;
+        if (listed) given = to_f32(reinterpret_cast<const T*>(a.x)[(size_t)row * a.ld + token]);
+    };
     auto result = [&](uint32_t row) {          // of a row whose sums and alternatives are in s and t
-        const T* const x = reinterpret_cast<const T*>(a.x) + (size_t)row * a.ld;
         const bool none = s.m == -INFINITY;
         if (s.m == INFINITY) s.z = NAN;        // Inf - Inf, as the formula has it
         const float logz = log1pf(s.z);
         auto log_of = [&](float y) { return y == -INFINITY && s.m == s.m && s.z == s.z ? -INFINITY : y - s.m - logz; };
         if (lane == 0) {
             if (a.entropy) a.entropy[row] = none ? 0.f : s.m == s.m ? logz - s.b / (1.f + s.z) : NAN;
-            if (a.tokens) {
-                const int32_t token = a.tokens[row];
-                a.logprob[row] = (uint32_t)token < a.n ? log_of(to_f32(x[token])) : 0.f;
-            }
+            if (a.tokens) a.logprob[row] = listed ? log_of(given) : 0.f;
         }
         if (TOP && lane < a.k) {
             a.top_ids[(size_t)row * a.k + lane] = (int32_t)~t.i;
@@ -482,16 +507,18 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
         for (uint32_t row = blockIdx.x / cluster;; turn++) {
             const Run r = run_of(row);
             const uint32_t half = turn & 1;
+            if (rank == 0) token_of(row);
             if (ok) ok = __all_sync(0xffffffffu, wait(there + 8 * half, (turn / 2) & 1));
             s = over_lanes(lane < kWarps ? part[half][lane] : Sums{-INFINITY, 0.f, 0.f});
             if constexpr (TOP) {
                 // The k lanes (of the block) with the largest entries have the k largest entries among theirs, whatever is larger than the k-th lane's: in the
                 // vector that holds the lane's largest, and where its others reach as high, in all of them.  (Order by value, then by vector: of equal
-                // values in one vector all are taken.)
-                t = lists[half][0][lane];
-                for (uint32_t w = 1; w < kWarps; w++) join(t, lists[half][w][lane]);
+                // values in one vector all are taken.)  The lanes' largest are in order already; what is found beside them, not much as a rule, is put in.
+                t = first_of(lists[half], a.k);
                 const Top least = {__shfl_sync(0xffffffffu, t.v, a.k - 1), __shfl_sync(0xffffffffu, t.i, a.k - 1)};
                 const uint4* const xv = reinterpret_cast<const uint4*>(r.x + r.head);
+                const bool mine = lane < a.k && t.v;
+                const uint32_t vec = ~t.i, of = mine ? (vec - r.v0) / kStageVecs % kWarps : 0, at = mine ? (vec - r.v0) % 32 : 0;
                 Top found = {0, 0};
                 auto offer = [&](float y, uint32_t vec, uint32_t id, bool in) {    // entry `id` of a lane's vector `vec`
                     const uint32_t o = order(y);
@@ -502,24 +529,31 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
                         insert(found, __shfl_sync(0xffffffffu, o, from), __shfl_sync(0xffffffffu, ~id, from));
                     }
                 };
-                auto offer_vector = [&](uint32_t vec, bool in) {
-                    const uint4 u = in ? xv[vec] : Vec<T>::nothing();
+                uint32_t first = 0xFFFFFFFFu;  // the lane's largest entry
+                auto offer_vector = [&](const uint4& u, uint32_t vec, uint32_t but, bool in) {
                     float v[N];
                     Vec<T>::unpack(u, v);
 #pragma unroll
-                    for (uint32_t e = 0; e < N; e++) offer(v[e], vec, r.head + vec * N + e, in);
+                    for (uint32_t e = 0; e < N; e++) offer(v[e], vec, r.head + vec * N + e, in && r.head + vec * N + e != but);
                 };
-                const bool mine = lane < a.k && t.v;
-                const uint32_t vec = ~t.i, of = mine ? (vec - r.v0) / kStageVecs % kWarps : 0, at = mine ? (vec - r.v0) % 32 : 0;
+                const uint4 own = mine && ok ? xv[vec] : Vec<T>::nothing();
+                if (mine && ok) {
+                    float v[N];
+                    Vec<T>::unpack(own, v);
+#pragma unroll
+                    for (uint32_t e = N; e > 0; e--)
+                        if (order(v[e - 1]) == t.v) first = r.head + vec * N + e - 1;
+                    found = Top{t.v, ~first};
+                }
                 const bool whole = mine && ok && seconds[half][of][at] >= least.v;
-                offer_vector(vec, mine && ok && !whole);
+                offer_vector(own, vec, first, mine && ok && !whole);
                 uint32_t again = __ballot_sync(0xffffffffu, whole);
                 while (again) {
-                    const uint32_t from = __ffs(again) - 1, f = r.v0 + __shfl_sync(0xffffffffu, of * kStageVecs + at, from);
+                    const uint32_t from = __ffs(again) - 1, f = r.v0 + __shfl_sync(0xffffffffu, of * kStageVecs + at, from), but = __shfl_sync(0xffffffffu, first, from);
                     again &= again - 1;
                     for (uint32_t j = lane; __any_sync(0xffffffffu, f + j / kAhead * kWarps * kStageVecs < r.v1); j += 32) {       // the lane's j-th vector
                         const uint32_t v = f + j / kAhead * kWarps * kStageVecs + j % kAhead * 32;
-                        offer_vector(v, v < r.v1);
+                        offer_vector(v < r.v1 ? xv[v] : Vec<T>::nothing(), v, but, v < r.v1);
                     }
                 }
                 // the entries outside of the vectors: those in front come before all others of their value, those behind after them
@@ -536,38 +570,27 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
             if (cluster > 1 || a.rows - row <= gridDim.x) break;
             row += gridDim.x;
         }
-        if (cluster > 1) {
-            if (lane == 0) all = s;
-            best[lane] = t;
+        if (cluster > 1) {                     // to the first block
+            if (lane == 0) {
+                const uint32_t to = cluster_map(smem_u32(&blocks[rank]), 0);
+                asm volatile("st.shared::cluster.f32 [%0], %1;\n st.shared::cluster.f32 [%0 + 4], %2;\n st.shared::cluster.f32 [%0 + 8], %3;" ::"r"(to), "f"(s.m), "f"(s.z), "f"(s.b) : "memory");
+            }
+            if (TOP) asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(cluster_map(smem_u32(&best[rank][lane]), 0)), "r"(t.v), "r"(t.i) : "memory");
         }
     }
     if (!ok && lane == 0 && a.status) atomicCAS(a.status, 0, 1);
-    if (cluster > 1) {                         // the blocks' results meet in the first one
+    if (cluster > 1) {
         __syncwarp();
         cluster_sync();
-        if (rank == 0) {
-            if (TOP) {                         // a warp has two or three blocks' lists, then one warp the warps'
-                if (warp < kWarps) {
-                    t = {0, 0};
-                    for (uint32_t w = warp; w < cluster; w += kWarps)
-                        join(t, Top{__float_as_uint(ld_cluster_f32(reinterpret_cast<const float*>(&best[lane].v), w)), __float_as_uint(ld_cluster_f32(reinterpret_cast<const float*>(&best[lane].i), w))});
-                    lists[0][warp][lane] = t;
-                }
-                __syncthreads();
-                if (warp == kWarps) {
-                    t = lists[0][0][lane];
-                    for (uint32_t w = 1; w < kWarps; w++) join(t, lists[0][w][lane]);
-                }
+        if (rank == 0 && warp == kWarps) {
+            if (TOP) {                         // a block's list a lane
+                uint32_t at = 0;
+                Top x = lane < cluster ? best[lane][0] : Top{0, 0};
+                t = largest(a.k, [&]() { return x; }, [&]() { x = ++at < 32 ? best[lane][at] : Top{0, 0}; });
             }
-            if (warp == kWarps) {
-                s = Sums{-INFINITY, 0.f, 0.f};
-                if (lane < cluster) s = Sums{ld_cluster_f32(&all.m, lane), ld_cluster_f32(&all.z, lane), ld_cluster_f32(&all.b, lane)};
-                s = over_lanes(s);
-                result(blockIdx.x / cluster);
-            }
+            s = over_lanes(lane < cluster ? blocks[lane] : Sums{-INFINITY, 0.f, 0.f});
+            result(blockIdx.x / cluster);
         }
-        __syncwarp();
-        cluster_sync();                        // the others' shared memory is read by then
     }
 }
 
