@@ -559,7 +559,9 @@ struct MergeArgs {
     const float *own_o, *own_ml, *pre_o, *pre_ml;
     bool shared;
 };
-constexpr uint32_t kMergeWarps = 8;
+// Sums of so many pieces are asked for at once: the registers for more of them cost warps that hide the rest (64 sequences with 1792 rows of pieces 43.9 us; with 5 44.4,
+// with 8 in blocks of 8 warps 46.0).
+constexpr uint32_t kMergeWarps = 4, kWideWarps = 16, kAsked = 4;
 
 // Sequence of a row, by a warp: 33 parts at a time.
 __device__ __forceinline__ uint32_t sequence_by_warp(const Cache& c, uint32_t row) {
@@ -576,7 +578,7 @@ __device__ __forceinline__ uint32_t sequence_by_warp(const Cache& c, uint32_t ro
 }
 
 template <typename T, int HD, bool WIDE>
-__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttnArgs a, const MergeArgs g) {
+__global__ void __launch_bounds__((WIDE ? kWideWarps : kMergeWarps) * 32) merge_kernel(const AttnArgs a, const MergeArgs g) {
     constexpr uint32_t E = HD / 32;
     const Cache& c = a.c;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -588,6 +590,24 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttnArgs 
     const Seq q = s < c.n_seqs ? sequence(c, s) : Seq{0, 0, 0};
     // the split kernel's plan, as far as it concerns this row; that of many entries it has left in the scratch
     uint32_t workers = 1, total = 0, pre_lo = c.shared, pre_hi = 0, before = 0, before_pre = 0;
+    const bool mine = token >= q.row0 && token < q.row0 + q.n;
+    // pieces of one entry: as many, from worker w0 on, or one that is whole
+    struct List {
+        uint32_t n, w0, beg, row;
+    };
+    auto list_of = [&](const Entry& u, uint32_t first, uint32_t i) {
+        List x{0, 0, 0, i % kRows};
+        if (u.steps == 0) return x;
+        x.beg = first + (head / c.group * u.tiles + i / kRows) * u.steps;
+        x.w0 = owner_of(x.beg, total, workers);
+        x.n = owner_of(x.beg + u.steps - 1, total, workers) - x.w0 + 1;
+        return x;
+    };
+    List own{g.own_parts, 0, 0, 0}, pre{g.pre_parts, 0, 0, 0};
+    auto look_up = [&]() {
+        own = list_of(entry_of(a, s, pre_lo, pre_hi), before, (token - q.row0) * c.group + head % c.group);
+        if (g.n_entries > c.n_seqs) pre = list_of(entry_of(a, c.n_seqs, pre_lo, pre_hi), before_pre, token * c.group + head % c.group);
+    };
     if (g.n_entries && g.n_entries <= kFewMerged) {
         if (g.n_entries > c.n_seqs) {
             seen_of(a, lane, 32, pre_lo, pre_hi);
@@ -605,37 +625,22 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttnArgs 
         before = __reduce_add_sync(0xffffffffu, before);
         before_pre = __reduce_add_sync(0xffffffffu, before_pre);
         workers = workers_of(total, g.most);
+        if (mine) look_up();
     }
     grid_dependency_wait();
     grid_launch_dependents();
-    if (token < q.row0 || token >= q.row0 + q.n) return;
-    // pieces of one entry: as many, from worker w0 on, or one that is whole
-    struct List {
-        uint32_t n, w0, beg, row;
-    };
-    auto list_of = [&](const Entry& u, uint32_t first, uint32_t i) {
-        List x{0, 0, 0, i % kRows};
-        if (u.steps == 0) return x;
-        x.beg = first + (head / c.group * u.tiles + i / kRows) * u.steps;
-        x.w0 = owner_of(x.beg, total, workers);
-        x.n = owner_of(x.beg + u.steps - 1, total, workers) - x.w0 + 1;
-        return x;
-    };
-    List own{g.own_parts, 0, 0, 0}, pre{g.pre_parts, 0, 0, 0};
-    if (g.n_entries) {
-        if (g.n_entries > kFewMerged) {
-            pre_lo = a.plan[0];
-            pre_hi = a.plan[1];
-            total = a.plan[2];
-            workers = a.plan[3];
-            before = a.plan[kPlanHead + s];
-            if (g.n_entries > c.n_seqs) before_pre = a.plan[kPlanHead + c.n_seqs];
-        }
-        own = list_of(entry_of(a, s, pre_lo, pre_hi), before, (token - q.row0) * c.group + head % c.group);
-        if (own.n == 1 && !g.shared) return;
-        if (g.n_entries > c.n_seqs) pre = list_of(entry_of(a, c.n_seqs, pre_lo, pre_hi), before_pre, token * c.group + head % c.group);
+    if (!mine) return;
+    if (g.n_entries > kFewMerged) {
+        pre_lo = a.plan[0];
+        pre_hi = a.plan[1];
+        total = a.plan[2];
+        workers = a.plan[3];
+        before = a.plan[kPlanHead + s];
+        if (g.n_entries > c.n_seqs) before_pre = a.plan[kPlanHead + c.n_seqs];
+        look_up();
     }
-    const uint32_t n = own.n + pre.n, step = WIDE ? kMergeWarps : 1;
+    if (g.n_entries && own.n == 1 && !g.shared) return;
+    const uint32_t n = own.n + pre.n, step = WIDE ? kWideWarps : 1;
     float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll
     for (uint32_t e = 0; e < E; e++) o[e] = 0.f;
@@ -659,9 +664,9 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttnArgs 
                 pml = y.ml + x.row * 2;
             }
         }
-        // the sums of the first eight are asked for along with the maxima
+        // the sums of the first ones are asked for along with the maxima
         const uint64_t at = reinterpret_cast<uint64_t>(po);
-        float v[8][E];
+        float v[kAsked][E];
         auto ask = [&](uint32_t k, float (&x)[E]) {
             const float* y = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, at, k & 31));
             if (k >= count) return;
@@ -674,7 +679,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttnArgs 
             }
         };
 #pragma unroll
-        for (uint32_t k = 0; k < 8; k++) ask(k, v[k]);
+        for (uint32_t k = 0; k < kAsked; k++) ask(k, v[k]);
         const float2 ml = pml ? *reinterpret_cast<const float2*>(pml) : make_float2(-INFINITY, 0.f);
         float top = fmaxf(m, ml.x);
 #pragma unroll
@@ -688,21 +693,21 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttnArgs 
         m = top;
 #pragma unroll
         for (uint32_t e = 0; e < E; e++) o[e] *= old;
-        for (uint32_t k0 = 0; k0 < count; k0 += 8) {
+        for (uint32_t k0 = 0; k0 < count; k0 += kAsked) {
 #pragma unroll
-            for (uint32_t k = 0; k < 8; k++) {
+            for (uint32_t k = 0; k < kAsked; k++) {
                 const float fk = __shfl_sync(0xffffffffu, f, (k0 + k) & 31);
                 if (k0 + k >= count) continue;
 #pragma unroll
                 for (uint32_t e = 0; e < E; e++) o[e] = fmaf(fk, v[k][e], o[e]);
             }
-            if (k0 + 8 < count)
+            if (k0 + kAsked < count)
 #pragma unroll
-                for (uint32_t k = 0; k < 8; k++) ask(k0 + 8 + k, v[k]);
+                for (uint32_t k = 0; k < kAsked; k++) ask(k0 + kAsked + k, v[k]);
         }
     }
     if constexpr (WIDE) {
-        __shared__ float sm[kMergeWarps], sl[kMergeWarps], so[kMergeWarps][HD];
+        __shared__ float sm[kWideWarps], sl[kWideWarps], so[kWideWarps][HD];
         if (lane == 0) { sm[warp] = m; sl[warp] = l; }
 #pragma unroll
         for (uint32_t e = 0; e < E; e++) so[warp][E * lane + e] = o[e];
@@ -710,12 +715,12 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttnArgs 
         if (warp > 0) return;
         float top = m;
 #pragma unroll
-        for (uint32_t w = 1; w < kMergeWarps; w++) top = fmaxf(top, sm[w]);
+        for (uint32_t w = 1; w < kWideWarps; w++) top = fmaxf(top, sm[w]);
         l = 0.f;
 #pragma unroll
         for (uint32_t e = 0; e < E; e++) o[e] = 0.f;
 #pragma unroll
-        for (uint32_t w = 0; w < kMergeWarps; w++) {
+        for (uint32_t w = 0; w < kWideWarps; w++) {
             const float f = top == -INFINITY ? 1.f : exp2_approx(sm[w] - top);
             l = fmaf(f, sl[w], l);
 #pragma unroll
@@ -833,7 +838,7 @@ static int32_t run(runit_ctx* ctx, const runit_paged_cfg* g, const runit_paged_b
     const MergeArgs m{c.n_entries, most, c.own_tc ? c.own_split : 0, c.pre_tc ? c.pre_split : 0, own.part_o, own.part_ml, pre.part_o, pre.part_ml, b->shared_len != 0};
     // a block for each where a segment has more pieces than a warp asks for at once, when all are alike
     const uint64_t pairs = (uint64_t)g->heads * b->rows;
-    if (share >= 16) runit_launch_chain(ctx, merge_kernel<T, HD, true>, dim3((uint32_t)pairs), dim3(kMergeWarps * 32), a, m);
+    if (share >= 16) runit_launch_chain(ctx, merge_kernel<T, HD, true>, dim3((uint32_t)pairs), dim3(kWideWarps * 32), a, m);
     else runit_launch_chain(ctx, merge_kernel<T, HD, false>, dim3((uint32_t)((pairs + kMergeWarps - 1) / kMergeWarps)), dim3(kMergeWarps * 32), a, m);
     return runit_after_launch(ctx, "paged_attention (merge)");
 }

@@ -1,12 +1,16 @@
 // Attention over a paged cache for many rows that share keys (prompts, and a prefix that a whole batch shares), on the tcgen05 tensor cores.
 //
 // A CTA has up to 256 (row, query head) pairs of one key head, as two tiles of 128, and walks a part of their positions in blocks of 128 that both tiles
-// share.  A tile's block: S = Q K^T into tensor memory (f32); four warps, a thread a row, take the maximum of S, form the weights 2^(s - ref) and put
-// them down as 16-bit numbers in columns of S that have been read; O += P V, accumulated in tensor memory, P being the A operand from there and V (as
-// it lies in the cache) MN-major.  That goes by halves of a block, 64 positions, each with columns of its own: while the weights of one are formed, the scores
-// of the next one are there already, and the products of the last one run (whole blocks: 3900 clocks a block of both tiles, halves 3700).  ref is a row's largest score until one exceeds it by 2^8, so that O
-// is rarely scaled; weights up to 2^8 keep the relative error of their rounding, and sums of them are f32.
-// Bound: exponentials (16 a clock and SM) and products (4096 multiply-adds a clock and SM) both take 2048 clocks for 256 rows x 128 positions x dim 128.
+// share.  By halves of a block, 64 positions, a tile has S = Q K^T in tensor memory (f32); four warps, a thread a row, read S (and free it for the next half),
+// take its maximum, form the weights 2^(s - ref) and put them down as 16-bit numbers in one of two places; O += P V, accumulated in tensor memory, P
+// being the A operand from there and V (as it lies in the cache) MN-major.  While the weights of one half are formed, the scores of the next one and the
+// product of the last one run.  ref is a row's largest score until one exceeds it by 2^8, so that O is rarely scaled; weights up to 2^8 keep the
+// relative error of their rounding, and sums of them are f32.
+// Tensor memory, 512 columns: S 64 and P 2 x 32 of each tile, O 128 of each.
+// Bound: products of 64 positions, whose operands from shared memory take 48 clocks instead of 32 (1260 a half for both tiles), and the warps of the softmax, which
+// have 512 clocks of exponentials a half and some 1200 with all the rest, two of them a scheduler.  3584 (row, head) pairs over 32768 positions, dim 128:
+// some 70 us, 860 TFLOP/s; prompts of 3 x 700 .. 2048 rows behind 2048 .. 4096 positions, 16 heads of 128, scores capped, 124 us, 500 TFLOP/s (256
+// tiles leave 148 SMs idle for a fifth of that: 38 blocks on the busiest, 30.8 on average).  Whole blocks of 128 positions at a time: 5% slower.
 // K and V of a block come by TMA as boxes of whole pages or of 128 positions; positions outside of what the CTA's rows see are zeros in V.
 #include "paged_attention.cuh"
 #include "tcgen05.cuh"
@@ -75,8 +79,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
     const Cache& c = a.c;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    // full, empty: one phase per use of a slot; s_full, p_full of a tile's halves: one per block; o_full, turn: one per half block; done: one
-    const uint32_t full = smem_u32(bars), empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots, p_full = s_full + 32, o_full = p_full + 32, done = o_full + 16, turn = done + 16;
+    // full, empty: one phase per use of a slot; p_full of a tile's halves: one per block; s_full, s_free, o_full, turn: one per half block; done: one
+    const uint32_t full = smem_u32(bars), empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots, s_free = s_full + 16, p_full = s_free + 16, o_full = p_full + 32, done = o_full + 16, turn = done + 16;
     if (tid == 0) {
         prefetch_map(&mk);
         prefetch_map(&mv);
@@ -211,11 +215,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
             mbar_init(o_full + 8 * i, 1);
             mbar_init(done + 8 * i, 1);
             mbar_init(turn + 8 * i, 4);
-        }
-        for (uint32_t i = 0; i < 4; i++) {
             mbar_init(s_full + 8 * i, 1);
-            mbar_init(p_full + 8 * i, 128);
+            mbar_init(s_free + 8 * i, 4);
         }
+        for (uint32_t i = 0; i < 4; i++) mbar_init(p_full + 8 * i, 128);
         fence_mbar_init();
     }
     __syncthreads();
@@ -247,9 +250,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
         // nothing is in flight when the block leaves
         mbar_drain(full, S::kSlots, n);
     } else if (warp >= kSoftWarps) {           // a tile's products
-        const uint32_t i = warp - kSoftWarps, qs = base + i * S::kTile, s_cols = tmem + 128 * i, o_cols = tmem + 256 + 128 * i;
+        const uint32_t i = warp - kSoftWarps, qs = base + i * S::kTile, s_cols = tmem + 64 * i, p_cols = tmem + 128 + 64 * i, o_cols = tmem + 256 + 128 * i;
         const uint32_t halves = i < chains ? 2 * n_blocks : 0;
-        uint32_t n_s[2] = {0, 0}, n_o = 0, n_d = 0;
+        uint32_t n_s = 0, n_o = 0, n_d = 0;
         auto slot_of_use = [&](uint32_t n) { return base + (2 + n % S::kSlots) * S::kTile; };
         auto wait = [&](uint32_t bar, uint32_t parity) {
             ok = ok && mbar_wait_timed(bar, parity, &abort_flag);
@@ -264,24 +267,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
 #pragma unroll
                 for (int s = 0; s < HD / 16; s++) {
                     const uint32_t off = (s >> 2) * S::kPanel + (s & 3) * 32;
-                    umma_bf16(s_cols + 64 * h, umma_desc_sw128(qs + off), umma_desc_sw128(kb + off), idesc_of<T>(128, kKeys / 2, 0), s > 0);
+                    umma_bf16(s_cols, umma_desc_sw128(qs + off), umma_desc_sw128(kb + off), idesc_of<T>(128, kKeys / 2, 0), s > 0);
                 }
-                umma_commit(s_full + 16 * i + 8 * h);
+                umma_commit(s_full + 8 * i);
                 if (h) umma_commit(empty + 8 * (n % S::kSlots));
             }
             __syncwarp();
-            n_s[h]++;
+            n_s++;
         };
         asm volatile("bar.sync 1, 320;" ::: "memory");           // Q is there
         tc_fence_after_sync();
         if (halves) {
             wait_full(0);
             if (ok) scores(0, 0);
-            if (ok) scores(0, 1);
         }
         for (uint32_t n = 0; n < halves && ok; n++) {
             const uint32_t j = n >> 1, h = n & 1, uv = 2 * j + 1, uk = 2 * j + 2, k0 = start + (b0 + j) * kKeys, vb = slot_of_use(uv);
             const bool last = n + 1 == halves;
+            if (!last) {                       // the next half's scores, as soon as this one's have been read
+                if (h) wait_full(uk);
+                wait(s_free + 8 * i, n & 1);
+                if (!ok) break;
+                scores(h ? uk : uk - 2, h ^ 1);
+            }
             if (h == 0) {
                 wait_full(uv);
                 if (!ok) break;
@@ -301,7 +309,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
             if (elect_one()) {
 #pragma unroll
                 for (int s = 0; s < 4; s++)
-                    umma_f16_ts(o_cols, s_cols + 64 * h + 8 * s, desc_mn_sw128(vb + (4 * h + s) * 2048, S::kPanel), idesc_of<T>(128, HD, 1), n > 0 || s > 0);
+                    umma_f16_ts(o_cols, p_cols + 32 * h + 8 * s, desc_mn_sw128(vb + (4 * h + s) * 2048, S::kPanel), idesc_of<T>(128, HD, 1), n > 0 || s > 0);
                 umma_commit(last ? done + 8 * i : o_full + 8 * i);
                 if (h && !last) umma_commit(empty + 8 * (uv % S::kSlots));
             }
@@ -311,17 +319,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
                 break;
             }
             n_o++;
-            if (n + 2 < halves) {
-                if (h == 0) wait_full(uk);
-                if (ok) scores(uk, h);
-            }
         }
-        mbar_drain(s_full + 16 * i, 1, n_s[0]);                  // nor is a product when the tensor memory goes back
-        mbar_drain(s_full + 16 * i + 8, 1, n_s[1]);
+        mbar_drain(s_full + 8 * i, 1, n_s);                      // nor is a product when the tensor memory goes back
         mbar_drain(o_full + 8 * i, 1, n_o);
         mbar_drain(done + 8 * i, 1, n_d);
     } else {
-        const uint32_t lanes = (warp & 3) << 21, s_cols = tmem + 128 * chain + lanes, o_cols = tmem + 256 + 128 * chain + lanes;
+        const uint32_t lanes = (warp & 3) << 21, s_cols = tmem + 64 * chain + lanes, p_cols = tmem + 128 + 64 * chain + lanes, o_cols = tmem + 256 + 128 * chain + lanes;
         const uint32_t limit = w.shared ? c.shared : 0x7FFFFFFFu;
         const uint32_t row_lo = !live ? 0 : max(w.shared ? 0 : c.shared, first_seen(pos, a.window)), row_hi = !live ? 0x7FFFFFFFu : min((uint32_t)max(0, pos + 1), limit);
         const float slope = a.slopes && live ? a.slopes[head] : 0.f;
@@ -352,16 +355,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
         bool cut = false;                      // some block had positions that this row does not see
         if (chain < chains) {
             for (uint32_t n = 0; n < 2 * n_blocks; n++) {
-                const uint32_t h = n & 1, k0 = start + (b0 + (n >> 1)) * kKeys + 64 * h, cols = s_cols + 64 * h;
-                if (ok) ok = mbar_wait_timed(s_full + 16 * chain + 8 * h, (n >> 1) & 1, &abort_flag);
+                const uint32_t h = n & 1, k0 = start + (b0 + (n >> 1)) * kKeys + 64 * h;
+                if (ok) ok = mbar_wait_timed(s_full + 8 * chain, n & 1, &abort_flag);
                 __syncwarp();
                 tc_fence_after_sync();
                 const bool inside = k0 >= row_lo && k0 + 64 <= row_hi;
                 cut |= !inside;
                 uint32_t r[2][32];
-                tmem_ld32(cols, r[0]);
-                tmem_ld32(cols + 32, r[1]);
+                tmem_ld32(s_cols, r[0]);
+                tmem_ld32(s_cols + 32, r[1]);
                 tmem_ld_wait();
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_free + 8 * chain);
                 // scores, of which `mul` times are in units of log2
                 if (!__all_sync(0xffffffffu, plain && inside && a.cap == 0.f)) {
 #pragma unroll
@@ -390,10 +396,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
                     for (int e = 0; e < 32; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(r[q][e]), __uint_as_float(r[q][e + 1]));
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
                 const bool rise = top > ref + kRise || (ref == -INFINITY && top > ref);
-                const float corr = rise ? exp2_approx(ref - top) : 1.f;
-                l *= corr;
-                ref = rise ? top : ref;
-                if (__any_sync(0xffffffffu, rise) && n > 0) {
+                const bool some = __any_sync(0xffffffffu, rise);
+                float corr = 1.f;
+                if (some) {
+                    corr = rise ? exp2_approx(ref - top) : 1.f;
+                    l *= corr;
+                    ref = rise ? top : ref;
+                }
+                if (some && n > 0) {
                     // O with the last half's product: the one before it is behind these scores, so one of two phases is on
                     if (ok) ok = mbar_wait_timed(o_full + 8 * chain, (n - 1) & 1, &abort_flag);
                     __syncwarp();
@@ -411,8 +421,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
                 const float sub = ref == -INFINITY ? 0.f : ref;
                 const uint64_t mul2 = packf(mul), sub2 = packf(-sub);
                 uint64_t both = 0;
-                // The tiles take their exponentials in turn (half n of the second one behind half n of the first, and that behind half n - 1 of the second).  Left
-                // alone they fall into step and do everything side by side (2900 clocks a half with a cap, 2500 in turn).
+                // The tiles take their exponentials in turn (half n of the second one once half n of the first is half done, and that behind half n - 1 of the
+                // second).  Left alone they fall into step and do everything side by side (3 to 7% slower).
                 if (ok && chains == 2 && (chain == 1 || n > 0)) ok = mbar_wait_timed(turn + 8 * chain, (chain == 1 ? n : n - 1) & 1, &abort_flag);
                 __syncwarp();
                 // The weights meet the values in the cache's type: half a step of it, relative, each; their sum is that of the 32-bit ones.
@@ -426,9 +436,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
                         both = fadd2(both, pack2(__float_as_uint(p0), __float_as_uint(p1)));
                         p[e] = Half2<T>::pack(p0, p1);
                     }
-                    tmem_st16(cols + 16 * q, p);
+                    tmem_st16(p_cols + 32 * h + 16 * q, p);
+                    if (q == 0 && lane == 0) mbar_arrive(turn + 8 * (chain ^ 1));
                 }
-                if (lane == 0) mbar_arrive(turn + 8 * (chain ^ 1));
                 tmem_st_wait();
                 tc_fence_before_sync();
                 mbar_arrive(p_full + 16 * chain + 8 * h);
