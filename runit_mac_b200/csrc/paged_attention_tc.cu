@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
             const uint32_t n = lane < c.n_seqs ? (sequence(c, lane).n * c.group + kTcRows - 1) / kTcRows : 0;
             if (index < __reduce_add_sync(0xffffffffu, n)) {
                 uint32_t r = 0;                // tiles of every sequence that come before the one that is looked for
-                for (uint32_t step = 1u << 23; step > 0; step /= 2)
+                for (uint32_t step = 1u << (31 - __clz(__reduce_max_sync(0xffffffffu, n))); step > 0; step /= 2)
                     if (__reduce_add_sync(0xffffffffu, min(n, r + step)) <= index) r += step;
                 const uint32_t rest = index - __reduce_add_sync(0xffffffffu, min(n, r)), has = __ballot_sync(0xffffffffu, n > r);
                 uint32_t e = has;
@@ -206,20 +206,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
             pos = (int32_t)q.len - (int32_t)(q.row0 + q.n - token);
         }
     }
-    if (tid == 0) {
-        for (uint32_t i = 0; i < S::kSlots; i++) {
-            mbar_init(full + 8 * i, 1);
-            mbar_init(empty + 8 * i, chains);
-        }
-        for (uint32_t i = 0; i < 2; i++) {
-            mbar_init(o_full + 8 * i, 1);
-            mbar_init(done + 8 * i, 1);
-            mbar_init(turn + 8 * i, 4);
-            mbar_init(s_full + 8 * i, 1);
-            mbar_init(s_free + 8 * i, 4);
-        }
-        for (uint32_t i = 0; i < 4; i++) mbar_init(p_full + 8 * i, 128);
+    // a barrier a lane
+    if (warp == kSoftWarps + 2) {
+        constexpr uint32_t n = 2 * S::kSlots;
+        const uint32_t i = lane - n;           // behind full and empty: s_full, s_free, p_full, o_full, done, turn
+        if (lane < n + 14) mbar_init(full + 8 * lane, lane < S::kSlots ? 1 : lane < n ? chains : i < 2 ? 1 : i < 4 ? 4 : i < 8 ? 128 : i < 12 ? 1 : 4);
         fence_mbar_init();
+    }
+    // Q, asked for before anything is waited for
+    constexpr uint32_t CH = HD / 8, RW = 32 / CH;                // 16-byte pieces of a row; rows that a warp reads at once
+    const uint32_t ch = lane % CH;
+    uint4 q_in[32 / RW];
+    if (warp < kSoftWarps) {
+#pragma unroll
+        for (uint32_t i = 0; i < 32 / RW; i++) {
+            const uint32_t r = i * RW + lane / CH, tk = __shfl_sync(0xffffffffu, token, r), hd = __shfl_sync(0xffffffffu, head, r);
+            const bool there = __shfl_sync(0xffffffffu, (int)live, r) != 0;
+            q_in[i] = there ? reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (size_t)tk * a.ldq + (size_t)hd * HD)[ch] : make_uint4(0, 0, 0, 0);
+        }
     }
     __syncthreads();
 
@@ -329,20 +333,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
         const uint32_t row_lo = !live ? 0 : max(w.shared ? 0 : c.shared, first_seen(pos, a.window)), row_hi = !live ? 0x7FFFFFFFu : min((uint32_t)max(0, pos + 1), limit);
         const float slope = a.slopes && live ? a.slopes[head] : 0.f;
         {
-            constexpr uint32_t CH = HD / 8, RW = 32 / CH;        // 16-byte pieces of a row; rows that a warp reads at once
             uint8_t* const dst = smem_raw + (base - smem_u32(smem_raw)) + chain * S::kTile + (warp & 3) * 32 * 128;
-            const uint32_t ch = lane % CH;
-            uint4 x[32 / RW];
-#pragma unroll
-            for (uint32_t i = 0; i < 32 / RW; i++) {
-                const uint32_t r = i * RW + lane / CH, tk = __shfl_sync(0xffffffffu, token, r), hd = __shfl_sync(0xffffffffu, head, r);
-                const bool there = __shfl_sync(0xffffffffu, (int)live, r) != 0;
-                x[i] = there ? reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (size_t)tk * a.ldq + (size_t)hd * HD)[ch] : make_uint4(0, 0, 0, 0);
-            }
 #pragma unroll
             for (uint32_t i = 0; i < 32 / RW; i++) {
                 const uint32_t r = i * RW + lane / CH;
-                *reinterpret_cast<uint4*>(dst + (ch >> 3) * S::kPanel + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x[i];
+                *reinterpret_cast<uint4*>(dst + (ch >> 3) * S::kPanel + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = q_in[i];
             }
             fence_proxy_async();
         }
