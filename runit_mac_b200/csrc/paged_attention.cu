@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
     float o[ND][4], m[2], l[2];
     // scores times mul are in units of log2; plain: products are scores times a positive scale.  Else they are scaled (before the cap or here) and biased.
     const bool plain = a.cap == 0.f && !a.slopes && a.scale > 0.f;
-    const float mul = plain ? a.scale * kLog2e : kLog2e, pre = a.cap != 0.f ? a.cap : a.scale, to_cap = a.cap != 0.f ? a.scale / a.cap : 0.f;
+    const float mul = plain ? a.scale * kLog2e : kLog2e, pre = a.cap != 0.f ? a.cap : a.scale;
     float slope[2];
     auto begin = [&]() {                       // rows of the reader's segment
 #pragma unroll
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
             const bool all = __all_sync(0xffffffffu, inside);
             float top[2] = {-INFINITY, -INFINITY};
             if (!plain || !all) {
-                if (a.cap != 0.f) tanh_scores(reinterpret_cast<float(&)[4 * NK]>(s), to_cap);
+                if (a.cap != 0.f) tanh_scores(reinterpret_cast<float(&)[4 * NK]>(s), a.tanh);
                 // in units of mul afterwards, like the plain ones
 #pragma unroll
                 for (uint32_t j = 0; j < NK; j++)
@@ -868,7 +868,7 @@ int32_t runit_paged_attention(runit_ctx_t* ctx, const runit_paged_cfg* cfg, cons
     const pg::Layout l = pg::layout_of(cfg, batch, c);
     if (scratch_bytes < l.bytes) return runit_fail(ctx, RUNIT_ERR_BUFFER_SIZE, "paged_attention: %zu bytes of scratch, %zu needed", scratch_bytes, l.bytes);
     uint8_t* const s = (uint8_t*)scratch;
-    const pg::AttnArgs a{pg::cache_of(ctx, cfg, batch), q, out, (const float*)cfg->slopes, ldq, ldo, cfg->window, cfg->scale, cfg->cap, (uint32_t*)(s + l.plan),
+    const pg::AttnArgs a{pg::cache_of(ctx, cfg, batch), q, out, (const float*)cfg->slopes, ldq, ldo, cfg->window, cfg->scale, cfg->cap, pg::tanh_of(cfg->cap != 0.f ? cfg->scale / cfg->cap : 0.f), (uint32_t*)(s + l.plan),
                          (float*)(s + l.slot_o), (float*)(s + l.slot_ml), (float*)(s + l.row_o), (float*)(s + l.row_ml), (float*)(s + l.pre_o), (float*)(s + l.pre_ml)};
     if (cfg->type == RUNIT_TYPE_F16) return cfg->dim == 128 ? pg::run<__half, 128>(ctx, cfg, batch, a, c, s, l) : pg::run<__half, 64>(ctx, cfg, batch, a, c, s, l);
     return cfg->dim == 128 ? pg::run<__nv_bfloat16, 128>(ctx, cfg, batch, a, c, s, l) : pg::run<__nv_bfloat16, 64>(ctx, cfg, batch, a, c, s, l);

@@ -11,6 +11,9 @@ namespace pg {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+struct Tanh {                // tanh_of
+    float k, far, n[3], f[4];                  // far: the square of v from which on neither polynomial serves
+};
 struct AttnArgs {
     Cache c;
     const void* q;
@@ -18,6 +21,7 @@ struct AttnArgs {
     const float* slopes;
     uint32_t ldq, ldo, window;
     float scale, cap;
+    Tanh tanh;               // of scale / cap times a product
     // scratch
     uint32_t* plan;          // kPlanHead words, then the steps in front of every entry
     float *slot_o, *slot_ml; // [2 * workers][16][dim] and [..][16][2]: pieces of segments that workers share
@@ -87,33 +91,55 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// tanh(k v) of N products, for a whole warp.  Below 0.5 tanh u = u p(u^2), p of degree 3 fitted to the least relative error there (weighted least squares,
-// 5.4e-7); a warp with a larger argument takes (1 - e^-2|u|) / (1 + e^-2|u|), off by some 2^-22.
-template <int N> __device__ __forceinline__ void tanh_scores(float (&v)[N], float k) {
-    uint64_t u[N / 2], w[N / 2];
-    const uint64_t k2 = packf(k);
+// tanh(k v) of N products.  tanh u = u p(u^2), p fitted to the least relative error (weighted least squares): of degree 2 below 0.25 (4.2e-7) and of degree 3
+// below 0.5 (5.5e-7); the powers of k are in the coefficients.  Larger arguments take (1 - e^-2|u|) / (1 + e^-2|u|), off by some 2^-22; so does their whole warp,
+// with u itself for those below 0.5, and every warp if powers of k leave the range.
+static inline Tanh tanh_of(float k_) {
+    const double k = k_, k2 = k * k;
+    const bool in = k2 > 0x1p-34 && k2 < 0x1p34;
+    Tanh h;
+    h.k = k_;
+    h.far = in ? (float)(0.25 / k2) : -1.f;
+    h.n[0] = (float)(0.9999996 * k); h.n[1] = (float)(-0.33321908 * k * k2); h.n[2] = (float)(0.12841612 * k * k2 * k2);
+    h.f[0] = (float)(0.99999946 * k); h.f[1] = (float)(-0.33326318 * k * k2); h.f[2] = (float)(0.13190296 * k * k2 * k2); h.f[3] = (float)(-0.04440222 * k * k2 * k2 * k2);
+    return h;
+}
+// For a whole warp, which looks first how large the arguments are.
+template <int N> __device__ __forceinline__ void tanh_scores(float (&v)[N], const Tanh& h) {
+    uint64_t x[N / 2], w[N / 2];
     float most = 0.f;
 #pragma unroll
     for (int i = 0; i < N / 2; i++) {
-        u[i] = fmul2(pack2(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1])), k2);
-        w[i] = fmul2(u[i], u[i]);
+        x[i] = pack2(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]));
+        w[i] = fmul2(x[i], x[i]);
         most = max3(most, __uint_as_float((uint32_t)w[i]), __uint_as_float((uint32_t)(w[i] >> 32)));
     }
-    if (__any_sync(0xffffffffu, most > 0.25f)) {
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const float x = v[i] * k, e = exp2_approx(-2.f * kLog2e * fabsf(x));
-            v[i] = copysignf(__fdividef(1.f - e, 1.f + e), x);
-        }
-    } else {
+    if (!__any_sync(0xffffffffu, most > h.far)) {
 #pragma unroll
         for (int i = 0; i < N / 2; i++) {
-            uint64_t p = ffma2(w[i], packf(-0.04440222f), packf(0.13190296f));
-            p = ffma2(w[i], p, packf(-0.33326318f));
-            p = fmul2(u[i], ffma2(w[i], p, packf(0.99999946f)));
+            const uint64_t p = fmul2(x[i], ffma2(w[i], ffma2(w[i], ffma2(w[i], packf(h.f[3]), packf(h.f[2])), packf(h.f[1])), packf(h.f[0])));
             v[2 * i] = __uint_as_float((uint32_t)p);
             v[2 * i + 1] = __uint_as_float((uint32_t)(p >> 32));
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float u = v[i] * h.k, u2 = u * u, e = exp2_approx(-2.f * kLog2e * fabsf(u));
+            const float small = u * fmaf(u2, fmaf(u2, fmaf(u2, -0.04440222f, 0.13190296f), -0.33326318f), 0.99999946f);
+            v[i] = u2 < 0.25f ? small : copysignf(__fdividef(1.f - e, 1.f + e), u);
+        }
+    }
+}
+// Below 0.25; beyond it the result exceeds kNearTanh, as u p(u^2) rises throughout (its derivative 1 - u^2 + 0.64 u^4 has no zero).  four: the largest magnitudes.
+constexpr float kNearTanh = 0.2449f;
+template <int N> __device__ __forceinline__ void tanh_near(float (&v)[N], const Tanh& h, float (&four)[4]) {
+#pragma unroll
+    for (int i = 0; i < N / 2; i++) {
+        const uint64_t x = pack2(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1])), w = fmul2(x, x);
+        const uint64_t p = fmul2(x, ffma2(w, ffma2(w, packf(h.n[2]), packf(h.n[1])), packf(h.n[0])));
+        v[2 * i] = __uint_as_float((uint32_t)p);
+        v[2 * i + 1] = __uint_as_float((uint32_t)(p >> 32));
+        four[i & 3] = max3(four[i & 3], fabsf(v[2 * i]), fabsf(v[2 * i + 1]));
     }
 }
 // The first position that the one at `pos` sees.

@@ -9,7 +9,7 @@
 // Tensor memory, 512 columns: S 64 and P 2 x 32 of each tile, O 128 of each.
 // Bound: products of 64 positions, whose operands from shared memory take 48 clocks instead of 32 (1260 a half for both tiles), and the warps of the softmax, which
 // have 512 clocks of exponentials a half and some 1200 with all the rest, two of them a scheduler.  3584 (row, head) pairs over 32768 positions, dim 128:
-// some 70 us, 860 TFLOP/s; prompts of 3 x 700 .. 2048 rows behind 2048 .. 4096 positions, 16 heads of 128, scores capped, 124 us, 500 TFLOP/s (256
+// some 70 us, 860 TFLOP/s; prompts of 3 x 700 .. 2048 rows behind 2048 .. 4096 positions, 16 heads of 128, scores capped, 117 us, 527 TFLOP/s (256
 // tiles leave 148 SMs idle for a fifth of that: 38 blocks on the busiest, 30.8 on average).  Whole blocks of 128 positions at a time: 5% slower.
 // K and V of a block come by TMA as boxes of whole pages or of 128 positions; positions outside of what the CTA's rows see are zeros in V.
 #include "paged_attention.cuh"
@@ -343,10 +343,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
         }
         asm volatile("bar.sync 1, 320;" ::: "memory");
         // plain: what the products (or their tanh) are multiplied by is positive, and nothing is added
-        const float pre = a.cap != 0.f ? a.cap : a.scale, to_cap = a.cap != 0.f ? a.scale / a.cap : 0.f;
+        const float pre = a.cap != 0.f ? a.cap : a.scale;
         const bool plain = !a.slopes && pre > 0.f;
         const float mul = plain ? pre * kLog2e : kLog2e;
         float ref = -INFINITY, l = 0.f;
+        bool wide = a.tanh.far < 0.f;          // some score is beyond the near polynomial
         bool cut = false;                      // some block had positions that this row does not see
         if (chain < chains) {
             for (uint32_t n = 0; n < 2 * n_blocks; n++) {
@@ -360,14 +361,32 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
                 tmem_ld32(s_cols, r[0]);
                 tmem_ld32(s_cols + 32, r[1]);
                 tmem_ld_wait();
+                if (a.cap != 0.f) {
+                    // The near polynomial grows with its argument, so that what comes out tells whether it was near: no vote ahead of it (7% of the time of the prompts
+                    // above).  Scores that were not are read again, and a warp that has met one looks first from then on.
+                    if (!wide) {
+                        float four[4] = {0.f, 0.f, 0.f, 0.f};
+                        tanh_near(reinterpret_cast<float(&)[32]>(r[0]), a.tanh, four);
+                        tanh_near(reinterpret_cast<float(&)[32]>(r[1]), a.tanh, four);
+                        wide = __any_sync(0xffffffffu, max3(fmaxf(four[0], four[1]), four[2], four[3]) > kNearTanh);
+                        if (wide) {
+                            tmem_ld32(s_cols, r[0]);
+                            tmem_ld32(s_cols + 32, r[1]);
+                            tmem_ld_wait();
+                        }
+                    }
+                    if (wide) {
+                        tanh_scores(reinterpret_cast<float(&)[32]>(r[0]), a.tanh);
+                        tanh_scores(reinterpret_cast<float(&)[32]>(r[1]), a.tanh);
+                    }
+                }
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_free + 8 * chain);
                 // scores, of which `mul` times are in units of log2
-                if (!__all_sync(0xffffffffu, plain && inside && a.cap == 0.f)) {
+                if (!__all_sync(0xffffffffu, plain && inside)) {
 #pragma unroll
                     for (uint32_t q = 0; q < 2; q++) {
-                        if (a.cap != 0.f) tanh_scores(reinterpret_cast<float(&)[32]>(r[q]), to_cap);
                         if (!plain) {
                             const float at_0 = -slope * (float)(pos - (int32_t)(k0 + 32 * q));
 #pragma unroll

@@ -36,6 +36,18 @@ def test_many_sequences(ctx, name):
     check(b, got, name)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 300])
+@pytest.mark.parametrize("cap,scale", [(10.0, None), (10.0, -0.125), (1e-4, None), (1e7, None), (50.0, 3.0)])
+def test_capped_scores_of_every_size(ctx, kind, rows, cap, scale):
+    """Keys that are small at first, then large, then small again, so that scores over the cap reach from 0.01 to 30 within one row; caps far below and far above them."""
+    b = Batch(rows, [(rows, 900)], 4, 2, 64, 32, kind, cap=cap, scale=scale)
+    for p in range(900):
+        b.k[b.table[0, p // 32], :, p % 32] *= 0.125 if p < 400 else 6.0 if 520 <= p < 530 else 1.0
+    b.k = rounded(b.k, kind)
+    check(b, b.attend(ctx))
+
+
 SOME = [dict(seqs=[(1, 700), (3, 40), (0, 0), (1, 5)], heads=14, kv_heads=2, dim=64, page=16, kind="f16"),
         dict(seqs=[(1, 320 + 9 * i) for i in range(30)], heads=8, kv_heads=2, dim=128, page=64, kind="bf16", shared=320),
         dict(seqs=[(150, 400), (130, 130)], heads=4, kv_heads=2, dim=128, page=32, kind="f16", cap=15.0)]
