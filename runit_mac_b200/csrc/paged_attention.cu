@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
     constexpr uint32_t KS = HD / 16, ND = HD / 8, NK = kStep / 8;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[kWarps * S::kStages];
-    __shared__ uint32_t sums[kWarps], edge[2];
+    __shared__ uint32_t sums[kWarps], edge[2], costs[kWarps][kFew];
     uint8_t* const ring = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
     uint32_t* const before = reinterpret_cast<uint32_t*>(ring + S::kRing);         // [n_entries + 1] steps in front of an entry
     const Cache& c = a.c;
@@ -176,13 +176,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
 #pragma unroll 1
         for (uint32_t k = 0; k < n_entries; k += 32) {
             v = k + lane < n_entries ? cost(k + lane) : 0;
+            costs[warp][k + lane] = v;
             total += __reduce_add_sync(0xffffffffu, v);
         }
         share();
         uint32_t at = 0;
 #pragma unroll 1
         for (uint32_t k = 0; k < n_entries; k += 32) {
-            if (n_entries > 32) v = k + lane < n_entries ? cost(k + lane) : 0;
+            if (n_entries > 32) v = costs[warp][k + lane];
             const uint32_t inc = scan(v) + at;
             if (n_entries > kFewMerged && blockIdx.x == 0 && warp == 0 && k + lane < n_entries) a.plan[kPlanHead + k + lane] = inc - v;
             const uint32_t here = __ballot_sync(0xffffffffu, v && x0 >= inc - v && x0 < inc);
@@ -337,8 +338,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
         for (uint32_t r = 0; r < 2; r++) {
             const uint32_t i = at.tile * kRows + g4 + 8 * r;
             live[r] = i < at.t.n * c.group;
-            const uint32_t token = at.t.row0 + (live[r] ? i / c.group : 0), head = at.h * c.group + (live[r] ? i % c.group : 0);
-            pos[r] = at.t.base + (int32_t)(i / c.group);
+            const uint32_t nth = at.t.n > 1 ? i / c.group : 0;   // (a division costs more than the rest of this)
+            const uint32_t token = at.t.row0 + (live[r] ? nth : 0), head = at.h * c.group + (live[r] ? i - nth * c.group : 0);
+            pos[r] = at.t.base + (int32_t)nth;
             uint32_t limit = 0x7FFFFFFFu;
             if (at.e >= c.n_seqs && live[r]) {
                 const uint32_t s = sequence_by_halves(c, token);
