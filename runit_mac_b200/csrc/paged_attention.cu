@@ -1,7 +1,9 @@
 // Attention of a batch of sequences over a paged cache: out_i = sum_j softmax_j(s_ij) v_j over the positions j that row i sees, s_ij = scale q_i . k_j,
 // then cap * tanh(s / cap), then minus slope * (i - j).
 //
-// Many rows that share keys: paged_attention_tc.cu.  Few rows a sequence (decoding): bound by HBM, which has to deliver every key and value once.  A segment is what shares keys: up to 16 (row, query head)
+// Many rows that share keys: paged_attention_tc.cu.  Few rows a sequence (decoding): bound by HBM, which has to deliver every key and value once (one row over
+// 131072 positions, 4 key heads of 128, f16: 268 MB in 51 us, 5.2 TB/s, of which 5 us are merge_kernel and 3 the way to the first copy; 64 sequences of
+// 60 to 8100 positions, 206 MB: 44 us, 4.7 TB/s).  A segment is what shares keys: up to 16 (row, query head)
 // pairs of one sequence and key head, and the positions that they see; the segments' steps of 32 positions, one behind the other, are dealt out evenly to
 // the warps of the grid, whatever the lengths.  A warp is on its own: it copies its steps by TMA into a ring (boxes of 16 positions, so that pages of
 // 16 are whole boxes), multiplies on the legacy tensor path with the rows as m16 (a tcgen05 tile would be 128 rows, mostly padding), and keeps
