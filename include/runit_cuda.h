@@ -645,7 +645,7 @@ typedef struct {
 int32_t runit_paged_append(runit_ctx_t*, const runit_paged_cfg* cfg, const runit_paged_batch* batch, const void* proj, int32_t proj_type, uint32_t ld,
                            const void* freq, uint32_t rot_dims, void* q_out, uint32_t ldq);
 /* out[row][head] = softmax over the positions that the row sees (those up to its own, within the window) of its scores, times their values.  q and out:
- * the cache's type, rows of ldq / ldo elements (multiples of 8), 16-byte aligned.  Scores, softmax and sums are f32; the weights are rounded to the cache's
+ * the cache's type, rows of ldq / ldo elements (multiples of 8), 16-byte aligned, not the same memory.  Scores, softmax and sums are f32; the weights are rounded to the cache's
  * type where they meet the values.  The shared positions are read once for all sequences.  A row that sees nothing gets zeros.  Values of positions that
  * a row does not see do not reach it, whatever they are.  scratch: 256-byte aligned, runit_paged_attention_scratch_bytes of it (which no two calls
  * in flight may share; it depends on the sizes in cfg and batch alone and needs no clearing). */

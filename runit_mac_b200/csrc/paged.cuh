@@ -63,6 +63,7 @@ static inline const char* why_not(const runit_paged_cfg* g, const runit_paged_ba
     if (g->page < 16 || g->page > 256 || (g->page & (g->page - 1)) != 0) return "page must be a power of two from 16 to 256";
     if (g->n_pages == 0 || g->n_pages > 0x7FFFFFFFu || (uint64_t)g->n_pages * g->kv_heads * g->page > 0x7FFFFFFFull) return "n_pages * kv_heads * page must be from 1 to 2^31 - 1";
     if (!std::isfinite(g->scale) || !std::isfinite(g->cap) || g->cap < 0.f) return "scale and cap must be finite, cap not negative";
+    if (g->cap != 0.f && !std::isfinite(g->scale / g->cap)) return "cap is too small for the scale";
     if (b->n_seqs == 0 || b->n_seqs > kMaxSeqs) return "n_seqs must be from 1 to 4096";
     if (b->rows == 0 || (uint64_t)b->rows * g->heads > 0x7FFFFFFFull) return "rows must not be 0, and rows * heads below 2^31";
     if (b->table_ld == 0 || (uint64_t)b->table_ld * g->page > 0x7FFFFFFFull) return "table_ld must not be 0, and table_ld * page below 2^31";

@@ -865,6 +865,7 @@ int32_t runit_paged_attention(runit_ctx_t* ctx, const runit_paged_cfg* cfg, cons
     if (!why) why = pg::why_not_memory(cfg, batch);
     RUNIT_REQUIRE(ctx, !why, "paged_attention: %s", why);
     RUNIT_REQUIRE(ctx, q && out && runit_aligned(q, 16) && runit_aligned(out, 16), "paged_attention: q and out must be 16-byte aligned");
+    RUNIT_REQUIRE(ctx, q != out, "paged_attention: q is read by several workers and must not be out");
     RUNIT_REQUIRE(ctx, ldq % 8 == 0 && ldo % 8 == 0 && ldq >= (uint64_t)cfg->heads * cfg->dim && ldo >= (uint64_t)cfg->heads * cfg->dim,
                   "paged_attention: ldq=%u, ldo=%u must be multiples of 8, rows of heads * dim at least", ldq, ldo);
     RUNIT_REQUIRE(ctx, scratch && runit_aligned(scratch, 256), "paged_attention: scratch must be 256-byte aligned");

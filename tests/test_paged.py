@@ -24,6 +24,11 @@ def test_descriptions_that_are_refused(change):
     assert _described(**change) == 0
 
 
+@pytest.mark.parametrize("cap,scale,fits", [(1e-40, 0.1, False), (1e-38, -3.0, True)])       # 3 / 1e-38 = 3e38 is below f32's largest, 3.4e38; 0.1 / 1e-40 = 1e39 is not
+def test_a_cap_that_the_scale_cannot_be_divided_by(cap, scale, fits):
+    assert (_described(cap=cap, scale=scale) > 0) == fits and _described(cap=1e-30, scale=scale) > 0
+
+
 def test_scratch_goes_with_the_sizes_alone():
     base = _described()
     assert base > 0 and _described() == base

@@ -48,6 +48,40 @@ def test_capped_scores_of_every_size(ctx, kind, rows, cap, scale):
     check(b, b.attend(ctx))
 
 
+@pytest.mark.parametrize("rows", [1, 140])
+@pytest.mark.parametrize("scale,slopes", [(0.0, None), (-0.2, None), (0.0, [0.3, -0.2, 0.0, 1.5])])
+def test_scales_that_are_not_positive(ctx, rows, scale, slopes):
+    """All scores alike (the mean of the values), the least product first, and a bias that alone decides."""
+    b = Batch(rows, [(rows, 300), (1, 33)], 4, 2, 128, 16, "f16", scale=scale, slopes=slopes)
+    check(b, b.attend(ctx))
+
+
+def test_attention_does_not_write_over_its_queries(ctx):
+    import runit_mac_b200 as R
+    b = Batch(2, [(1, 20)], 4, 2, 64, 16, "f16")
+    keep, cfg, batch = b.upload(ctx)
+    n = R.paged_attention_scratch_bytes(ctx, cfg, batch)
+    q, scratch, before = ctx.new_buffer(4096), ctx.new_buffer(n), ctx.launches
+    with pytest.raises(R.KernelError) as e:
+        R.paged_attention(ctx, C.byref(cfg), C.byref(batch), q, 256, q, 256, scratch, n)
+    assert e.value.status == 2 and ctx.launches == before
+
+
+def test_append_over_the_projected_queries(ctx):
+    """Queries of the cache's type may go back to where they were: the same as to rows of their own."""
+    import runit_mac_b200 as R
+    b = Batch(3, [(40, 50), (1, 20)], 6, 2, 64, 16, "bf16", poison=1.0)
+    row, freq = (6 + 4) * 64, 1e4 ** (-2.0 * np.arange(32) / 64)
+    fb = ctx.buffer_from(np.stack([freq.astype(np.float32), (freq - freq.astype(np.float32)).astype(np.float32)]))
+    proj = to_bits(np.random.default_rng(2).normal(0, 1, (b.rows, row)), "bf16")
+    keep, cfg, batch = b.upload(ctx)
+    p, q = ctx.buffer_from(proj), ctx.new_buffer(b.rows * 6 * 64 * 2)
+    R.paged_append(ctx, C.byref(cfg), C.byref(batch), p, R.TYPE_BF16, row, fb, 64, q, 6 * 64)
+    R.paged_append(ctx, C.byref(cfg), C.byref(batch), p, R.TYPE_BF16, row, fb, 64, p, row)
+    ctx.flush()
+    np.testing.assert_array_equal(p.download(np.uint16, b.rows * row).reshape(b.rows, row)[:, :6 * 64], q.download(np.uint16, b.rows * 6 * 64).reshape(b.rows, 6 * 64))
+
+
 SOME = [dict(seqs=[(1, 700), (3, 40), (0, 0), (1, 5)], heads=14, kv_heads=2, dim=64, page=16, kind="f16"),
         dict(seqs=[(1, 320 + 9 * i) for i in range(30)], heads=8, kv_heads=2, dim=128, page=64, kind="bf16", shared=320),
         dict(seqs=[(150, 400), (130, 130)], heads=4, kv_heads=2, dim=128, page=32, kind="f16", cap=15.0)]
