@@ -739,20 +739,21 @@ __global__ void __launch_bounds__((WIDE ? kWideWarps : kMergeWarps) * 32) merge_
 
 // ── which kernel has which positions, and the scratch ──
 // By the (row, query head) pairs that share keys: up to 16 (a tile of the split kernel) it is bound by the copies, beyond that it reads its keys again for every
-// 16.  The parts of the kernel for many rows: as many as fill 148 SMs best, of four blocks at least.
+// 16.  The parts of the kernel for many rows: as many as take the least time, which is that of a part (its blocks, and four more for what it takes to begin and to
+// end) as often as the parts go round 148 SMs, a tenth of a block a part for the sums, and five blocks for the merge where there is none with one part.
+// (40 pairs behind 9216 shared positions: 18 parts 21 us, one 131; 288 behind 18816: 29 parts 29 us, 25 of them 34; two prompts of 700 rows behind a window
+// of 143, 16 heads: one part 25 us, three 59; 250 rows, 32 heads, without anything in front: one part 16 us, two 22.)
 struct Choice {
     bool own_tc, pre_tc, direct;
     uint32_t own_tiles, pre_tiles, own_split, pre_split, n_entries;
 };
-static uint32_t parts_of(uint64_t ctas, uint64_t blocks) {
+static uint32_t parts_of(uint64_t ctas, uint64_t blocks, double apart) {
     uint32_t best = 1;
-    double most = 0.0;
-    for (uint32_t z = 1; z <= 64 && (z == 1 || z * 4ull <= blocks); z++) {
-        const uint64_t n = ctas * z, waves = (n + 147) / 148;
-        if (z > 1 && n > 2 * 148) break;
-        const double fill = (double)n / (148.0 * (double)waves) - 0.01 * z;         // a part costs its prologue and its sums
-        if (fill > most) {
-            most = fill;
+    double least = 1e30;
+    for (uint32_t z = 1; z <= 64 && (z == 1 || z <= blocks); z++) {
+        const double took = (double)((ctas * z + 147) / 148) * (double)((blocks + z - 1) / z + 4) + 0.1 * z + (z > 1 ? apart : 0.0);
+        if (took < least) {
+            least = took;
             best = z;
         }
     }
@@ -765,8 +766,9 @@ static Choice choose(const runit_paged_cfg* g, const runit_paged_batch* b) {
     c.pre_tc = b->shared_len && pairs > 16;
     c.own_tiles = (uint32_t)(pairs / 256 + b->n_seqs);
     c.pre_tiles = (uint32_t)((pairs + 255) / 256);
-    c.own_split = parts_of((pairs / 256 + (b->n_seqs + 1) / 2) * g->kv_heads, (uint64_t)b->table_ld * g->page / 128);
-    c.pre_split = parts_of((uint64_t)c.pre_tiles * g->kv_heads, b->shared_len / 128);
+    const uint64_t all = (uint64_t)b->table_ld * g->page, seen = g->window ? min(all, (uint64_t)g->window + 256) : all;
+    c.own_split = parts_of((pairs / 256 + (b->n_seqs + 1) / 2) * g->kv_heads, (seen + 127) / 128, b->shared_len ? 0.0 : 5.0);
+    c.pre_split = parts_of((uint64_t)c.pre_tiles * g->kv_heads, b->shared_len / 128, 0.0);
     c.direct = c.own_tc && !b->shared_len && c.own_split == 1;
     c.n_entries = c.own_tc ? 0 : b->n_seqs + (b->shared_len && !c.pre_tc ? 1 : 0);       // (own_tc: more than 32 pairs, so pre_tc as well)
     return c;
