@@ -739,7 +739,9 @@ __global__ void __launch_bounds__((WIDE ? kWideWarps : kMergeWarps) * 32) merge_
 
 // ── which kernel has which positions, and the scratch ──
 // By the (row, query head) pairs that share keys: up to 16 (a tile of the split kernel) it is bound by the copies, beyond that it reads its keys again for every
-// 16.  The parts of the kernel for many rows: as many as take the least time, which is that of a part (its blocks, and four more for what it takes to begin and to
+// 16, from the second-level cache.  Where that makes fewer than eight steps a worker, it is done before a launch of the other kernel would be: 40 pairs behind 9216
+// positions 13 us and 21, 238 behind 384 with 4 key heads 14 and 20; at 18 steps a worker (288 pairs behind 18816) it is 37 and 29.  (Rows of a sequence's
+// own go to the other kernel from 32 pairs on, however few: 45 rows 12 us and 19.)  The parts of the kernel for many rows: as many as take the least time, which is that of a part (its blocks, and four more for what it takes to begin and to
 // end) as often as the parts go round 148 SMs, a tenth of a block a part for the sums, and five blocks for the merge where there is none with one part.
 // (40 pairs behind 9216 shared positions: 18 parts 21 us, one 131; 288 behind 18816: 29 parts 29 us, 25 of them 34; two prompts of 700 rows behind a window
 // of 143, 16 heads: one part 25 us, three 59; 250 rows, 32 heads, without anything in front: one part 16 us, two 22.)
@@ -763,7 +765,8 @@ static Choice choose(const runit_paged_cfg* g, const runit_paged_batch* b) {
     const uint64_t group = g->heads / g->kv_heads, pairs = b->rows * group;
     Choice c;
     c.own_tc = pairs > 32ull * b->n_seqs;
-    c.pre_tc = b->shared_len && pairs > 16;
+    const uint64_t pre_steps = (pairs + 15) / 16 * g->kv_heads * (b->shared_len / kStep);
+    c.pre_tc = b->shared_len && pairs > 16 && (c.own_tc || pre_steps > 8ull * kWarps * 148);
     c.own_tiles = (uint32_t)(pairs / 256 + b->n_seqs);
     c.pre_tiles = (uint32_t)((pairs + 255) / 256);
     const uint64_t all = (uint64_t)b->table_ld * g->page, seen = g->window ? min(all, (uint64_t)g->window + 256) : all;

@@ -36,6 +36,47 @@ def test_many_sequences(ctx, name):
     check(b, got, name)
 
 
+BEHIND = {
+    "single rows": dict(seqs=[(1, 512 + 1 + 11 * i % 60) for i in range(300)], heads=16, kv_heads=4, dim=64, page=16, kind="f16", shared=512),
+    "drafts, cap, bias": dict(seqs=[(3, 512 + 3 + 7 * i % 50) for i in range(60)], heads=32, kv_heads=4, dim=128, page=64, kind="bf16", shared=512, cap=20.0, slopes=[0.1 / (i + 1) for i in range(32)]),
+    "a window that reaches back": dict(seqs=[(1, 1024 + 9 * i % 500) for i in range(90)], heads=32, kv_heads=2, dim=64, page=32, kind="f16", shared=1024, window=700, extra_rows=2),
+    "some end inside": dict(seqs=[(1, 1 + 37 * i % 511) if i % 3 == 0 else (i % 4, 512 + 5 * i % 90) for i in range(160)], heads=32, kv_heads=2, dim=128, page=128, kind="f16", shared=512),
+}
+
+
+@pytest.mark.parametrize("name", BEHIND)
+def test_many_rows_behind_shared_positions(ctx, name):
+    """Enough of both that the kernel for many rows takes the shared ones: three launches."""
+    b = Batch(sum(map(ord, name)), **BEHIND[name])
+    before = ctx.launches
+    got = b.attend(ctx)
+    assert ctx.launches - before == 3
+    assert (got[b.n_rows:] == rounded(-3.0, b.kind)).all()
+    check(b, got, name)
+
+
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+def test_values_behind_shared_positions_that_a_row_does_not_see(ctx, value):
+    """Rows that end inside the shared positions do not see what comes after them there; the others carry it."""
+    b = Batch(3, [(1, 100 + i) if i % 2 else (1, 1024 + 1 + i % 30) for i in range(100)], 32, 2, 64, 16, "f16", shared=1024)
+    clean, bound = b.reference()
+    b.v[b.table[0, 300 // 16], 0, 300 % 16, 5] = value
+    b.k[b.table[0, 400 // 16], 1, 400 % 16, 3] = np.nan
+    before = ctx.launches
+    got = b.attend(ctx)
+    assert ctx.launches - before == 3
+    for r, (_, n) in enumerate(b.seqs):
+        for h in range(32):
+            x, ref, off = got[r, h].astype(np.float64), clean[r, h], bound[r, h]
+            if h // 16 == 1 and n > 400:
+                assert np.isnan(x).all()
+                continue
+            if h // 16 == 0 and n > 300:
+                assert not np.isfinite(x[5])
+                x, ref, off = np.delete(x, 5), np.delete(ref, 5), np.delete(off, 5)
+            assert (np.abs(x - ref) <= off + 2.0 ** -25).all(), (r, h)
+
+
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
 @pytest.mark.parametrize("rows", [1, 300])
 @pytest.mark.parametrize("cap,scale", [(10.0, None), (10.0, -0.125), (1e-4, None), (1e7, None), (50.0, 3.0)])
