@@ -60,6 +60,32 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
     __shared__ float cs[kMaxRot / 2], sn[kMaxRot / 2];
     const Cache& c = a.c;
     const uint32_t row = blockIdx.x, tid = threadIdx.x, half = a.rot / 2, dim = c.dim;
+    const uint32_t first = a.q_out ? 0 : c.heads, turned = c.heads + c.kv_heads, all = turned + c.kv_heads;
+    const TP* x = reinterpret_cast<const TP*>(a.proj) + (size_t)row * a.ld;
+    // items of 16 values, kAppendItems a thread at a time; the first ones are asked for ahead of the way to their pages
+    const uint32_t per = dim / 16, n = (all - first) * per, pairs = a.rot / 16;
+    struct Item {
+        uint32_t head, lo;
+        bool turn;
+    };
+    auto item_of = [&](uint32_t i) {
+        const uint32_t head = first + i / per, d = i % per;
+        const bool turn = head < turned && d < pairs;
+        return Item{head, turn ? 8 * d : head < turned ? a.rot + 16 * (d - pairs) : 16 * d, turn};
+    };
+    float u[kAppendItems][8], v[kAppendItems][8];
+    auto ask = [&](uint32_t i0) {
+#pragma unroll
+        for (uint32_t e = 0; e < kAppendItems; e++) {
+            const uint32_t i = i0 + e * kAppendThreads + tid;
+            if (i >= n) break;
+            const Item it = item_of(i);
+            const TP* p = x + (size_t)it.head * dim;
+            load8(p + it.lo, u[e]);
+            load8(p + (it.turn ? it.lo + half : it.lo + 8), v[e]);
+        }
+    };
+    if constexpr (VEC) ask(0);
     const uint32_t s = sequence_of(c, row);
     if (s >= c.n_seqs) return;
     const Seq q = sequence(c, s);
@@ -71,7 +97,6 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
     const uint32_t pos = q.len - back;
     bool ok;
     const size_t at = page_row(c, c.table + (size_t)s * c.table_ld, pos, 0, &ok);
-    const TP* x = reinterpret_cast<const TP*>(a.proj) + (size_t)row * a.ld;
     TC *kc = reinterpret_cast<TC*>(c.k) + at, *vc = reinterpret_cast<TC*>(c.v) + at, *qo = reinterpret_cast<TC*>(a.q_out) + (size_t)row * a.ldq;
     const size_t head_stride = (size_t)dim << c.page_log2;
     // where head i of the row goes; null: nowhere
@@ -82,50 +107,34 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
         return i < c.kv_heads ? kc + i * head_stride : vc + (i - c.kv_heads) * head_stride;
     };
     if (tid < half) ls::sincos_at(pos, a.freq[tid], a.freq[half + tid], &sn[tid], &cs[tid]);
-    const uint32_t first = a.q_out ? 0 : c.heads, turned = c.heads + c.kv_heads, all = turned + c.kv_heads;
+    __syncthreads();
     if constexpr (VEC) {
-        const uint32_t per = dim / 16, n = (all - first) * per, pairs = a.rot / 16;
-        float u[kAppendItems][8], v[kAppendItems][8];
         for (uint32_t i0 = 0; i0 < n; i0 += kAppendThreads * kAppendItems) {
+            if (i0 > 0) ask(i0);
 #pragma unroll
             for (uint32_t e = 0; e < kAppendItems; e++) {
                 const uint32_t i = i0 + e * kAppendThreads + tid;
                 if (i >= n) break;
-                const uint32_t head = first + i / per, d = i % per;
-                const TP* p = x + (size_t)head * dim;
-                const bool turn = head < turned && d < pairs;
-                const uint32_t lo = turn ? 8 * d : head < turned ? a.rot + 16 * (d - pairs) : 16 * d;
-                load8(p + lo, u[e]);
-                load8(p + (turn ? lo + half : lo + 8), v[e]);
-            }
-            if (i0 == 0) __syncthreads();
-#pragma unroll
-            for (uint32_t e = 0; e < kAppendItems; e++) {
-                const uint32_t i = i0 + e * kAppendThreads + tid;
-                if (i >= n) break;
-                const uint32_t head = first + i / per, d = i % per;
-                TC* t = target(head);
+                const Item it = item_of(i);
+                TC* t = target(it.head);
                 if (!t) continue;
-                const bool turn = head < turned && d < pairs;
-                const uint32_t lo = turn ? 8 * d : head < turned ? a.rot + 16 * (d - pairs) : 16 * d;
-                if (turn) {
+                if (it.turn) {
                     float y[8], z[8];
 #pragma unroll
                     for (uint32_t j = 0; j < 8; j++) {
-                        const float co = cs[lo + j], si = sn[lo + j];
+                        const float co = cs[it.lo + j], si = sn[it.lo + j];
                         y[j] = fmaf(u[e][j], co, -(v[e][j] * si));
                         z[j] = fmaf(u[e][j], si, v[e][j] * co);
                     }
-                    store8(t + lo, y);
-                    store8(t + lo + half, z);
+                    store8(t + it.lo, y);
+                    store8(t + it.lo + half, z);
                 } else {
-                    store8(t + lo, u[e]);
-                    store8(t + lo + 8, v[e]);
+                    store8(t + it.lo, u[e]);
+                    store8(t + it.lo + 8, v[e]);
                 }
             }
         }
     } else {
-        __syncthreads();
         const uint32_t per = dim / 2, n = (all - first) * per;
         for (uint32_t i = tid; i < n; i += kAppendThreads) {
             const uint32_t head = first + i / per, d = i % per;
