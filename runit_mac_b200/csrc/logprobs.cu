@@ -23,7 +23,7 @@ struct Args {
     uint32_t ld, n, k, rows;
 };
 
-constexpr uint32_t kThreads = 256, kWarps = kThreads / 32 - 1, kAhead = 4, kStages = 3;     // kWarps read; one more adds up what they have found
+constexpr uint32_t kWarps = 7, kAhead = 4, kStages = 3;     // kWarps read; one or two more add up what they have found
 constexpr uint32_t kStageVecs = 32 * kAhead, kStageBytes = 16 * kStageVecs, kBlocksPerSm = 4;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kLeast = -200.f;      // e^-200 is 0 in f32
 
@@ -366,9 +366,10 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
 
 // A block takes rows blockIdx.x / cluster, + gridDim.x, ...; with few rows a cluster of `cluster` blocks (a power of two up to 16) shares one, and the first of them
 // adds up.  Seven warps read: the row's 16-byte vectors go to them in turn, 128 at a time, which come by a bulk copy of 2 KB into the warp's ring of three,
-// and a warp goes on to the next row when it is through; the eighth warp turns what they have found into the row's results, one row behind.
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(const Args a, const uint32_t cluster) {
+// and a warp goes on to the next row when it is through; the eighth warp (and a ninth, in turn)
+// turns what they have found into the row's results, one row behind.
+template <typename T, bool TOP, uint32_t ADDERS>
+__global__ void __launch_bounds__(32 * (kWarps + ADDERS), kBlocksPerSm) token_logprobs_kernel(const Args a, const uint32_t cluster) {
     constexpr uint32_t N = Vec<T>::N;
     extern __shared__ __align__(128) uint8_t ring[];             // [kWarps][kStages][kStageBytes]
     __shared__ __align__(8) uint64_t bars[kWarps * kStages + 4];
@@ -503,8 +504,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
             a.top_logprobs[(size_t)row * a.k + lane] = log_of(value(t.v));
         }
     };
-    if (warp == kWarps) {
-        for (uint32_t row = blockIdx.x / cluster;; turn++) {
+    if (ADDERS == 1 ? warp == kWarps : warp >= kWarps && (warp == kWarps || a.rows - blockIdx.x > gridDim.x)) {
+        turn = warp - kWarps;                  // row after row in turn
+        for (uint32_t row = blockIdx.x / cluster + turn * gridDim.x;; turn += ADDERS) {
             const Run r = run_of(row);
             const uint32_t half = turn & 1;
             if (rank == 0) token_of(row);
@@ -567,8 +569,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
             __syncwarp();
             if (lane == 0) mbar_arrive(taken + 8 * half);
             if (cluster == 1) result(row);
-            if (cluster > 1 || a.rows - row <= gridDim.x) break;
-            row += gridDim.x;
+            if (cluster > 1 || a.rows - row <= (uint64_t)ADDERS * gridDim.x) break;
+            row += ADDERS * gridDim.x;
         }
         if (cluster > 1) {                     // to the first block
             if (lane == 0) {
@@ -600,19 +602,19 @@ static uint32_t cluster_of(uint32_t rows, uint32_t n) {
     while (c < 16 && (uint64_t)rows * c * 2 <= 2 * 148 && n / (c * 2) >= 2048) c *= 2;
     return c;
 }
-template <typename T, bool TOP> static int32_t run(runit_ctx* ctx, const Args& a) {
+template <typename T, bool TOP, uint32_t ADDERS> static int32_t launch(runit_ctx* ctx, const Args& a) {
     constexpr uint32_t smem = kWarps * kStages * kStageBytes;
     const uint32_t cluster = cluster_of(a.rows, a.n);
     static bool configured[64] = {false};
     if (ctx->device >= 64 || !configured[ctx->device]) {
-        RUNIT_CUDA_TRY(ctx, cudaFuncSetAttribute(token_logprobs_kernel<T, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        RUNIT_CUDA_TRY(ctx, cudaFuncSetAttribute(token_logprobs_kernel<T, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        RUNIT_CUDA_TRY(ctx, cudaFuncSetAttribute(token_logprobs_kernel<T, TOP, ADDERS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        RUNIT_CUDA_TRY(ctx, cudaFuncSetAttribute(token_logprobs_kernel<T, TOP, ADDERS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         if (ctx->device < 64) configured[ctx->device] = true;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(cluster > 1 ? a.rows * cluster : min(a.rows, (uint32_t)ctx->sm_count * kBlocksPerSm));
     cfg.dynamicSmemBytes = smem;
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(32 * (kWarps + ADDERS));
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -622,8 +624,15 @@ template <typename T, bool TOP> static int32_t run(runit_ctx* ctx, const Args& a
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = ctx->tune.pdl != 0 ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, TOP>, a, cluster);           // errors surface in runit_after_launch
+    cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, TOP, ADDERS>, a, cluster);           // errors surface in runit_after_launch
     return runit_after_launch(ctx, "token_logprobs");
+}
+// A second warp to add up where blocks have rows one behind the other and short ones, so that the alternatives take as long as the reading (4000 rows of 2000, 20
+// alternatives: 64 us with one, 45 with two; 2048 rows of 152064 with 5: 119 and 122).
+template <typename T, bool TOP> static int32_t run(runit_ctx* ctx, const Args& a) {
+    if constexpr (TOP)
+        if (a.rows > (uint32_t)ctx->sm_count * kBlocksPerSm && a.n < 32768) return launch<T, TOP, 2>(ctx, a);
+    return launch<T, TOP, 1>(ctx, a);
 }
 
 }  // namespace lp
