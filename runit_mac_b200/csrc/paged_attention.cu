@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
             }
 #pragma unroll
             for (uint32_t d = 0; d < ND; d++) *reinterpret_cast<float2*>(po + 8 * d + 2 * t4) = make_float2(o[d][2 * r], o[d][2 * r + 1]);
-            if (t4 == 0) *reinterpret_cast<float2*>(pml) = make_float2(m[r], l[r]);
+            if (t4 == 0) *reinterpret_cast<float2*>(pml) = make_float2(m[r] - Half2<T>::kLift, l[r]);      // what the sums are relative to
         }
     };
 
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
                     o[d][3] *= corr[1];
                 }
             }
-            const float sub[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+            const float sub[2] = {m[0] == -INFINITY ? 0.f : m[0] - Half2<T>::kLift, m[1] == -INFINITY ? 0.f : m[1] - Half2<T>::kLift};
             // the product's rounding against that of the maximum (2^-24 of the score) stays in the weight, as an f32 score's own would
 #pragma unroll
             for (uint32_t j = 0; j < NK; j++)
@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
 #pragma unroll
                 for (uint32_t i = 0; i < 2; i++)
                     seen[i] = (ka + 8 * i >= at.lo && ka + 8 * i < at.hi ? 0x8000u : 0) | (ka + 8 * i + 1 >= at.lo && ka + 8 * i + 1 < at.hi ? 0x80000000u : 0);
-                // the weights meet the values in the cache's type: half a step of it, relative, each; their sum is that of the 32-bit ones
+                // the weights meet the values in the cache's type: half a step of it, relative, each (Half2: how far down); their sum is that of the 32-bit ones
                 const uint32_t pa[4] = {Half2<T>::pack(s[2 * k][0], s[2 * k][1]), Half2<T>::pack(s[2 * k][2], s[2 * k][3]), Half2<T>::pack(s[2 * k + 1][0], s[2 * k + 1][1]),
                                         Half2<T>::pack(s[2 * k + 1][2], s[2 * k + 1][3])};
                 const uint32_t row = ((lane >> 3) & 1) * 8 + (lane & 7);
@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
     }
 }
 
-// Adds up what the launches have left of a (row, query head): a warp for each, or a block (WIDE) where a segment has many pieces.  A lane has the maximum and sum
+// Adds up what the launches have left of a (row, query head): a warp for each, or a block (WIDE) where a segment has many pieces.  A lane has the reference and sum
 // of a piece, the factors 2^(m - max m) go round, and every lane adds up 2 or 4 of the dimensions.  Rows that a worker has written itself are left.
 struct MergeArgs {
     uint32_t n_entries, most;                  // of the split kernel, and its workers at most: no entries when it has not run (all sequences, and the shared positions if their rows are few)

@@ -55,9 +55,14 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory"); }
-// What differs between the two 16-bit types: products, packing, and bits that are no number.
+// What differs between the two 16-bit types: products, packing, bits that are no number, and their range.  Weights 2^(s - ref) are rounded to the type with ref
+// kLift below the row's largest score (the kernel for many rows: kLift - kRise, and a score may exceed ref + that by kRise before ref follows).  f16 has ten bits
+// down to 2^-14 only and nothing below 2^-25: with the largest weights at 2^15, those down to 2^-29 of the largest (2^-25 in the other kernel) are rounded by half a step
+// relative to themselves, and 131072 weights below that, 2^-8 of the sum at most, by 2^-19 of it together.  With the largest at 1 a row whose best key is 17 nats ahead of
+// thousands of others lost up to all that those others have.  bf16 has its eight bits throughout.
 template <typename T> struct Half2;
 template <> struct Half2<__half> {
+    static constexpr float kLift = 15.f, kRise = 4.f;
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __half2 h = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
@@ -71,6 +76,7 @@ template <> struct Half2<__half> {
     }
 };
 template <> struct Half2<__nv_bfloat16> {
+    static constexpr float kLift = 0.f, kRise = 8.f;
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);

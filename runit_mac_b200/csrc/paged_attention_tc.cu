@@ -4,8 +4,8 @@
 // share.  By halves of a block, 64 positions, a tile has S = Q K^T in tensor memory (f32); four warps, a thread a row, read S (and free it for the next half),
 // take its maximum, form the weights 2^(s - ref) and put them down as 16-bit numbers in one of two places; O += P V, accumulated in tensor memory, P
 // being the A operand from there and V (as it lies in the cache) MN-major.  While the weights of one half are formed, the scores of the next one and the
-// product of the last one run.  ref is a row's largest score until one exceeds it by 2^8, so that O is rarely scaled; weights up to 2^8 keep the
-// relative error of their rounding, and sums of them are f32.
+// product of the last one run.  ref is a row's largest score until one exceeds it by 2^kRise, so that O is rarely scaled; the weights keep the
+// relative error of their rounding (Half2), and sums of them are f32.
 // Tensor memory, 512 columns: S 64 and P 2 x 32 of each tile, O 128 of each.
 // Bound: products of 64 positions, whose operands from shared memory take 48 clocks instead of 32 (1260 a half for both tiles), and the warps of the softmax, which
 // have 512 clocks of exponentials a half and some 1200 with all the rest, two of them a scheduler.  3584 (row, head) pairs over 32768 positions, dim 128:
@@ -19,7 +19,6 @@ namespace runit {
 namespace pg {
 
 constexpr uint32_t kTcRows = 256, kKeys = 128, kSoftWarps = 8, kTcThreads = 32 * (kSoftWarps + 3);   // and a warp for each tile's products, one for copies
-constexpr float kRise = 8.f;                       // log2 of what a weight may exceed 1 by
 
 template <int HD> struct TcShape {
     static constexpr uint32_t kPanel = 128 * 128;  // 64 elements of 128 rows
@@ -72,6 +71,7 @@ __device__ __noinline__ float2 plain_row(const AttnArgs& a, const int32_t* table
 template <typename T, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const AttnArgs a, const TcArgs w) {
     using S = TcShape<HD>;
+    constexpr float kRise = Half2<T>::kRise, kBelow = Half2<T>::kLift > kRise ? Half2<T>::kLift - kRise : 0.f;       // what weights are relative to: ref - kBelow
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[2 * S::kSlots + 14];
     __shared__ uint32_t tmem_holder, found[4], sums[kTcThreads / 32];
@@ -432,14 +432,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
                         tmem_st16(o_cols + 16 * q, o);
                     }
                 }
-                const float sub = ref == -INFINITY ? 0.f : ref;
+                const float sub = ref == -INFINITY ? 0.f : ref - kBelow;
                 const uint64_t mul2 = packf(mul), sub2 = packf(-sub);
                 uint64_t both = 0;
                 // The tiles take their exponentials in turn (half n of the second one once half n of the first is half done, and that behind half n - 1 of the
                 // second).  Left alone they fall into step and do everything side by side (3 to 7% slower).
                 if (ok && chains == 2 && (chain == 1 || n > 0)) ok = mbar_wait_timed(turn + 8 * chain, (chain == 1 ? n : n - 1) & 1, &abort_flag);
                 __syncwarp();
-                // The weights meet the values in the cache's type: half a step of it, relative, each; their sum is that of the 32-bit ones.
+                // The weights meet the values in the cache's type: half a step of it, relative, each (Half2: how far down); their sum is that of the 32-bit ones.
 #pragma unroll
                 for (uint32_t q = 0; q < 2; q++) {
                     uint32_t p[16];
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
                     }
                 }
             }
-            if (live && ok && !w.direct) *reinterpret_cast<float2*>(pml) = make_float2(ref, l);
+            if (live && ok && !w.direct) *reinterpret_cast<float2*>(pml) = make_float2(ref - kBelow, l);
             uint32_t again = __ballot_sync(0xffffffffu, live && ok && odd && cut);
             while (again) {
                 const uint32_t from = __ffs(again) - 1;
