@@ -43,6 +43,7 @@ __device__ __forceinline__ size_t page_row(const Cache& c, const int32_t* table,
 // Rows and length of a sequence, within the tensors.  A sequence without rows is not looked at further.
 struct Seq {
     uint32_t row0, n, len;
+    bool falls;                                 // its rows would end before they begin, so that others overlap
 };
 __device__ __forceinline__ Seq sequence(const Cache& c, uint32_t s) {
     const int32_t a = c.q_start[s], b = c.q_start[s + 1], n = c.kv_len[s], cap = (int32_t)min((uint64_t)c.table_ld << c.page_log2, (uint64_t)0x7FFFFFFF);
@@ -51,6 +52,7 @@ __device__ __forceinline__ Seq sequence(const Cache& c, uint32_t s) {
     const uint32_t end = (uint32_t)max(0, min(b, (int32_t)c.rows));
     q.n = end > q.row0 ? end - q.row0 : 0;
     q.len = (uint32_t)max(0, min(n, cap));
+    q.falls = b < a;
     if (a < 0 || b < a || (uint32_t)b > c.rows || (q.n > 0 && (n < (int32_t)q.n || n > cap))) report(c);
     return q;
 }

@@ -37,11 +37,12 @@ struct Entry {
 // Three more than its positions take, about what beginning and ending a segment costs a worker (64 sequences of 60 to 8100 positions: 113000 clocks for those
 // with eight segments, 83000 for those with one; 77 us without, 64 with one step more, 60 with three).
 __device__ __forceinline__ uint32_t steps_of(uint32_t lo, uint32_t hi) { return hi > lo ? (hi - (lo & ~(kBox - 1)) + kStep - 1) / kStep + 3 : 0; }
-__device__ __forceinline__ Entry entry_of(const AttnArgs& a, uint32_t e, uint32_t pre_lo, uint32_t pre_hi) {
+__device__ __forceinline__ Entry entry_of(const AttnArgs& a, uint32_t e, uint32_t pre_lo, uint32_t pre_hi, bool& falls) {
     const Cache& c = a.c;
     Entry t;
     if (e < c.n_seqs) {
         const Seq s = sequence(c, e);
+        falls |= s.falls;
         t.row0 = s.row0;
         t.n = s.n;
         t.base = (int32_t)s.len - (int32_t)s.n;
@@ -60,9 +61,19 @@ __device__ __forceinline__ Entry entry_of(const AttnArgs& a, uint32_t e, uint32_
     t.steps = steps_of(t.lo, t.hi);
     return t;
 }
-__device__ __forceinline__ uint32_t cost_of(const AttnArgs& a, uint32_t e, uint32_t pre_lo, uint32_t pre_hi) {
-    const Entry t = entry_of(a, e, pre_lo, pre_hi);
+__device__ __forceinline__ Entry entry_of(const AttnArgs& a, uint32_t e, uint32_t pre_lo, uint32_t pre_hi) {
+    bool falls = false;
+    return entry_of(a, e, pre_lo, pre_hi, falls);
+}
+// Where starts fall (sequence() reports it), sequences overlap, and their steps can be too many for 32 bits: shares of a wrapped count would lie anywhere.  Whoever
+// counts the steps learns of it here, and deals out nothing.
+__device__ __forceinline__ uint32_t cost_of(const AttnArgs& a, uint32_t e, uint32_t pre_lo, uint32_t pre_hi, bool& falls) {
+    const Entry t = entry_of(a, e, pre_lo, pre_hi, falls);
     return t.tiles * t.steps * a.c.kv_heads;
+}
+__device__ __forceinline__ uint32_t cost_of(const AttnArgs& a, uint32_t e, uint32_t pre_lo, uint32_t pre_hi) {
+    bool falls = false;
+    return cost_of(a, e, pre_lo, pre_hi, falls);
 }
 // The shared positions that some row of sequences e, e + step, ... sees.
 __device__ __forceinline__ void seen_of(const AttnArgs& a, uint32_t e, uint32_t step, uint32_t& lo, uint32_t& hi) {
@@ -158,6 +169,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
         x1 = me < workers && total ? begin_of(me + 1, total, workers) : 0;
     };
     auto cost = [&](uint32_t e) { return cost_of(a, e, pre_lo, pre_hi); };
+    bool falls = false;
     auto scan = [&](uint32_t v) {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -177,10 +189,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
         uint32_t v = 0;
 #pragma unroll 1
         for (uint32_t k = 0; k < n_entries; k += 32) {
-            v = k + lane < n_entries ? cost(k + lane) : 0;
+            v = k + lane < n_entries ? cost_of(a, k + lane, pre_lo, pre_hi, falls) : 0;
             costs[warp][k + lane] = v;
             total += __reduce_add_sync(0xffffffffu, v);
         }
+        falls = __any_sync(0xffffffffu, falls);
         share();
         uint32_t at = 0;
 #pragma unroll 1
@@ -208,7 +221,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
         uint32_t sum = 0;
         for (uint32_t e = beg; e < end; e++) {
             before[e] = sum;
-            sum += cost(e);
+            sum += cost_of(a, e, pre_lo, pre_hi, falls);
         }
         const uint32_t inc = scan(sum);
         if (lane == 31) sums[warp] = inc;
@@ -220,7 +233,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
             if (blockIdx.x == 0) a.plan[kPlanHead + e] = before[e];
         }
         if (tid == kWarps * 32 - 1) before[n_entries] = off + sum;
-        __syncthreads();
+        falls = __syncthreads_or(falls);
         total = before[n_entries];
         share();
         uint32_t l = 0, r = n_entries;         // the last entry that begins at or before x0 (those without steps come before it)
@@ -235,10 +248,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_split_kernel(const __gri
     if (n_entries > kFewMerged && blockIdx.x == 0 && tid == 0) {
         a.plan[0] = pre_lo;
         a.plan[1] = pre_hi;
-        a.plan[2] = total;
+        a.plan[2] = falls ? 0 : total;
         a.plan[3] = workers;
     }
-    if (x0 == x1) return;
+    if (x0 == x1 || falls) return;             // (a count of 0 instead took 6 more registers, and 2.4 us of 131072 positions)
 
     // A place in the order of steps.  Reader and copier walk it, the copier kStages ahead.
     struct Cursor {
@@ -601,7 +614,7 @@ __global__ void __launch_bounds__((WIDE ? kWideWarps : kMergeWarps) * 32) merge_
     };
     auto list_of = [&](const Entry& u, uint32_t first, uint32_t i) {
         List x{0, 0, 0, i % kRows};
-        if (u.steps == 0) return x;
+        if (u.steps == 0 || total == 0) return x;
         x.beg = first + (head / c.group * u.tiles + i / kRows) * u.steps;
         x.w0 = owner_of(x.beg, total, workers);
         x.n = owner_of(x.beg + u.steps - 1, total, workers) - x.w0 + 1;
@@ -618,14 +631,15 @@ __global__ void __launch_bounds__((WIDE ? kWideWarps : kMergeWarps) * 32) merge_
             pre_lo = __reduce_min_sync(0xffffffffu, pre_lo);
             pre_hi = __reduce_max_sync(0xffffffffu, pre_hi);
         }
+        bool falls = false;
 #pragma unroll 1
         for (uint32_t k = lane; k < g.n_entries; k += 32) {
-            const uint32_t v = cost_of(a, k, pre_lo, pre_hi);
+            const uint32_t v = cost_of(a, k, pre_lo, pre_hi, falls);
             total += v;
             if (k < s) before += v;
             if (k < c.n_seqs) before_pre += v;
         }
-        total = __reduce_add_sync(0xffffffffu, total);
+        total = __any_sync(0xffffffffu, falls) ? 0 : __reduce_add_sync(0xffffffffu, total);
         before = __reduce_add_sync(0xffffffffu, before);
         before_pre = __reduce_add_sync(0xffffffffu, before_pre);
         workers = workers_of(total, g.most);
