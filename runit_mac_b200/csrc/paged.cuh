@@ -43,6 +43,7 @@ __device__ __forceinline__ size_t page_row(const Cache& c, const int32_t* table,
 // Rows and length of a sequence, within the tensors.  A sequence without rows is not looked at further.
 struct Seq {
     uint32_t row0, n, len;
+    int32_t given;                              // the length as it stands there
     bool falls;                                 // its rows would end before they begin, so that others overlap
 };
 __device__ __forceinline__ Seq sequence(const Cache& c, uint32_t s) {
@@ -52,6 +53,7 @@ __device__ __forceinline__ Seq sequence(const Cache& c, uint32_t s) {
     const uint32_t end = (uint32_t)max(0, min(b, (int32_t)c.rows));
     q.n = end > q.row0 ? end - q.row0 : 0;
     q.len = (uint32_t)max(0, min(n, cap));
+    q.given = n;
     q.falls = b < a;
     if (a < 0 || b < a || (uint32_t)b > c.rows || (q.n > 0 && (n < (int32_t)q.n || n > cap))) report(c);
     return q;

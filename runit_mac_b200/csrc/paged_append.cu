@@ -90,11 +90,12 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
     if (s >= c.n_seqs) return;
     const Seq q = sequence(c, s);
     const uint32_t back = q.row0 + q.n - row;                    // rows up to the sequence's end, this one included
-    if (row < q.row0 || row >= q.row0 + q.n || back > q.len) {   // starts that do not rise, or more rows than positions
-        report(c);
+    // By the length as it stands there: by one that is cut to the table, rows would move onto positions that others have.
+    const uint32_t pos = (uint32_t)q.given - back;
+    if (row < q.row0 || row >= q.row0 + q.n || back > q.len || (q.given != (int32_t)q.len && pos >= c.table_ld << c.page_log2)) {
+        report(c);                                               // starts that do not rise, more rows than positions, or a position behind the table
         return;
     }
-    const uint32_t pos = q.len - back;
     bool ok;
     const size_t at = page_row(c, c.table + (size_t)s * c.table_ld, pos, 0, &ok);
     TC *kc = reinterpret_cast<TC*>(c.k) + at, *vc = reinterpret_cast<TC*>(c.v) + at, *qo = reinterpret_cast<TC*>(a.q_out) + (size_t)row * a.ldq;

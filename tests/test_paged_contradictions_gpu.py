@@ -4,7 +4,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from paged_batches import Batch, check
+from paged_batches import Batch, check, from_bits, to_bits
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +31,37 @@ def test_starts_that_fall_and_would_be_more_work_than_can_be_counted(ctx, n_seqs
     assert e.value.status == 2 and "paged cache" in str(e.value)
     b = Batch(6, [(1, 90), (2, 200), (1, 70)], 4, 2, 64, 16, "bf16")
     check(b, b.attend(ctx), "afterwards")
+
+
+def _append(ctx, b, proj):
+    """Pages and queries that an append without rotation leaves, and whether it was reported."""
+    import runit_mac_b200 as R
+    keep, cfg, batch = b.upload(ctx)
+    q = ctx.buffer_from(to_bits(np.full((b.rows, b.heads * b.dim), -3.0), b.kind))
+    R.paged_append(ctx, C.byref(cfg), C.byref(batch), ctx.buffer_from(proj), R.TYPE_F32, proj.shape[1], None, 0, q, b.heads * b.dim)
+    told = False
+    try:
+        ctx.flush()
+    except R.KernelError as e:
+        assert e.status == 2 and "paged cache" in str(e)
+        told = True
+    k, v = (from_bits(keep[n].download(np.uint16, b.k.size), b.kind).reshape(b.k.shape) for n in ("k", "v"))
+    return k, v, from_bits(q.download(np.uint16, b.rows * b.heads * b.dim), b.kind).reshape(b.rows, b.heads, b.dim), told
+
+
+@pytest.mark.parametrize("beyond", [0, 1, 2, 3, 40, 2 ** 30])
+def test_an_append_behind_the_table_leaves_the_positions_in_front(ctx, beyond):
+    """Three rows of a sequence whose length exceeds its pages: those with a place go there, the others nowhere; no other position changes."""
+    b = Batch(3, [(2, 20), (3, 64), (1, 9)], 2, 1, 64, 16, "f16", poison=5.0, table_extra=0)
+    proj = b.rng.normal(0, 1, (6, 256)).astype(np.float32)
+    b.kv_len[1] = 64 + beyond
+    k, v, q, told = _append(ctx, b, proj)
+    assert told == (beyond > 0)
+    x = from_bits(to_bits(proj, "f16"), "f16").reshape(6, 4, 64)
+    want_k, want_v, want_q = b.k.copy(), b.v.copy(), np.full((6, 2, 64), -3.0)
+    for s, r, p in ((0, 0, 18), (0, 1, 19), (1, 2, 61 + beyond), (1, 3, 62 + beyond), (1, 4, 63 + beyond), (2, 5, 8)):
+        if p < 64:
+            want_q[r] = x[r, :2]
+            want_k[b.table[s, p // 16], :, p % 16], want_v[b.table[s, p // 16], :, p % 16] = x[r, 2:3], x[r, 3:]
+    for got, want in ((k, want_k), (v, want_v), (q, want_q)):
+        np.testing.assert_array_equal(got, want)
