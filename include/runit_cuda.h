@@ -641,7 +641,8 @@ typedef struct {
 /* Projected rows [q: heads x dim | k, v: kv_heads x dim] of ld elements (proj_type f32 or the cache's type): the first rot_dims coordinates of q and
  * k are rotated (pairs (i, i + rot_dims / 2), angle position * (freq[0][i] + freq[1][i]), freq f32 [2][rot_dims / 2] as for the retention; rot_dims
  * 0: none), k and v go to the pages of their positions, q to q_out (rows of ldq elements of the cache's type; NULL: keys and values only).  f32
- * arithmetic, rounded once.  A page that gets rows belongs to one sequence. */
+ * arithmetic, rounded once.  A page that gets rows belongs to one sequence, but for the shared ones: rows of shared positions go to the pages of table row 0, whichever
+ * sequence they come with (rows of several sequences at one position hold the same). */
 int32_t runit_paged_append(runit_ctx_t*, const runit_paged_cfg* cfg, const runit_paged_batch* batch, const void* proj, int32_t proj_type, uint32_t ld,
                            const void* freq, uint32_t rot_dims, void* q_out, uint32_t ldq);
 /* out[row][head] = softmax over the positions that the row sees (those up to its own, within the window) of its scores, times their values.  q and out:

@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
         return;
     }
     bool ok;
-    const size_t at = page_row(c, c.table + (size_t)s * c.table_ld, pos, 0, &ok);
+    const size_t at = page_row(c, c.table + (pos < c.shared ? 0 : (size_t)s * c.table_ld), pos, 0, &ok);      // shared positions: in the first sequence's pages
     TC *kc = reinterpret_cast<TC*>(c.k) + at, *vc = reinterpret_cast<TC*>(c.v) + at, *qo = reinterpret_cast<TC*>(a.q_out) + (size_t)row * a.ldq;
     const size_t head_stride = (size_t)dim << c.page_log2;
     // where head i of the row goes; null: nowhere

@@ -65,3 +65,21 @@ def test_an_append_behind_the_table_leaves_the_positions_in_front(ctx, beyond):
             want_k[b.table[s, p // 16], :, p % 16], want_v[b.table[s, p // 16], :, p % 16] = x[r, 2:3], x[r, 3:]
     for got, want in ((k, want_k), (v, want_v), (q, want_q)):
         np.testing.assert_array_equal(got, want)
+
+
+@pytest.mark.parametrize("entries", ["none", "others"])
+def test_an_append_at_shared_positions_goes_to_the_pages_of_the_first_sequence(ctx, entries):
+    """Sequences that end inside the shared positions, or whose rows begin there; what their own table rows hold for those positions is not looked at, be it no
+    page or one of another sequence."""
+    b = Batch(5, [(2, 40), (3, 33), (2, 20), (1, 60)], 2, 1, 64, 16, "bf16", shared=32, poison=5.0)
+    b.table[1:, :2] = -7 if entries == "none" else b.table[[0, 0, 0], [2, 2, 2]][:, None]
+    proj = b.rng.normal(0, 1, (8, 256)).astype(np.float32)
+    k, v, q, told = _append(ctx, b, proj)
+    assert not told
+    x = from_bits(to_bits(proj, "bf16"), "bf16").reshape(8, 4, 64)
+    want_k, want_v = b.k.copy(), b.v.copy()
+    for s, r, p in ((0, 0, 38), (0, 1, 39), (0, 2, 30), (0, 3, 31), (1, 4, 32), (0, 5, 18), (0, 6, 19), (3, 7, 59)):
+        want_k[b.table[s, p // 16], :, p % 16], want_v[b.table[s, p // 16], :, p % 16] = x[r, 2:3], x[r, 3:]
+    np.testing.assert_array_equal(k, want_k)
+    np.testing.assert_array_equal(v, want_v)
+    np.testing.assert_array_equal(q, x[:, :2])
