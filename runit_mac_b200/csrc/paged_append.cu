@@ -2,7 +2,7 @@
 //
 // y_i = x_i cos a_i - x_{i+h} sin a_i, y_{i+h} = x_i sin a_i + x_{i+h} cos a_i for i < h = rot_dims / 2, a_i = position * freq_i.  The position is an
 // integer and freq_i the sum of two floats, so that the angle of a far position keeps its 24 bits (a product of two floats loses as many as the
-// position has).  One rounding, at the end.
+// position has); from 2^17 on it is formed in 64 bits.  One rounding, at the end.
 // Bound: HBM (every value is read once and written once: 7167 rows of 16 + 32 heads of 128 from f32, 264 MB, in 46 us; a block per row of 192 threads that ask for
 // their 128 bytes each before anything else; 128 threads with 4 such pieces 3 more); latency for a few rows.
 #include "linear_state.cuh"
@@ -39,6 +39,14 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float (
 #pragma unroll
     for (int i = 0; i < 8; i++) e[i] = from_f32<T>(v[i]);
     *reinterpret_cast<uint4*>(p) = u;
+}
+
+// Sine and cosine of the angle of a position from 2^17 on: the turn by what the f32 product was rounded by, which the near ones take, is of the second order, and
+// short by 4e-7 at 2^18 and 2e-3 at 2^22; from 2^24 on the position itself is no f32.
+__device__ __noinline__ float2 sincos_far(uint32_t pos, float hi, float lo) {
+    double s, c;
+    sincos((double)pos * ((double)hi + (double)lo), &s, &c);
+    return make_float2((float)s, (float)c);
 }
 
 // The sequence of a row (as many as have ended at or before it), by all threads of the block; c.n_seqs: nobody's row.
@@ -107,7 +115,14 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
         i -= c.heads;
         return i < c.kv_heads ? kc + i * head_stride : vc + (i - c.kv_heads) * head_stride;
     };
-    if (tid < half) ls::sincos_at(pos, a.freq[tid], a.freq[half + tid], &sn[tid], &cs[tid]);
+    if (tid < half) {
+        if (pos < 1u << 17) ls::sincos_at(pos, a.freq[tid], a.freq[half + tid], &sn[tid], &cs[tid]);
+        else {
+            const float2 t = sincos_far(pos, a.freq[tid], a.freq[half + tid]);
+            sn[tid] = t.x;
+            cs[tid] = t.y;
+        }
+    }
     __syncthreads();
     if constexpr (VEC) {
         for (uint32_t i0 = 0; i0 < n; i0 += blockDim.x * kAppendItems) {
