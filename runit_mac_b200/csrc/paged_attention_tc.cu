@@ -35,37 +35,77 @@ template <> __host__ __device__ constexpr uint32_t idesc_of<__half>(uint32_t m, 
 template <> __host__ __device__ constexpr uint32_t idesc_of<__nv_bfloat16>(uint32_t m, uint32_t n, uint32_t b_mn) { return umma_idesc_f16(m, n, b_mn) | (1u << 7) | (1u << 10); }
 
 // One row's attention over positions lo .. hi of a table, by a warp with plain arithmetic: for rows whose products met a value that is no number at a
-// position that they do not see (0 x Inf).  Returns maximum (log2 units) and sum; o: HD / 32 of the dimensions per lane.
+// position that they do not see (0 x Inf).  A lane takes the score of one of 32 positions, then the warp their values one by one.  Returns maximum (log2 units)
+// and sum; o: HD / 32 of the dimensions per lane.
 template <typename T, int HD>
 __device__ __noinline__ float2 plain_row(const AttnArgs& a, const int32_t* table, uint32_t token, uint32_t head, int32_t pos, uint32_t lo, uint32_t hi, float* out) {
     constexpr uint32_t E = HD / 32;
     const Cache& c = a.c;
     const uint32_t lane = threadIdx.x & 31;
-    const T* qp = reinterpret_cast<const T*>(a.q) + (size_t)token * a.ldq + (size_t)head * HD + lane * E;
-    float x[E], o[E], m = -INFINITY, l = 0.f;
+    const uint4* const qp = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (size_t)token * a.ldq + (size_t)head * HD);
+    float o[E], m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (uint32_t e = 0; e < E; e++) { x[e] = to_f32(qp[e]); o[e] = 0.f; }
+    for (uint32_t e = 0; e < E; e++) o[e] = 0.f;
     const float slope = a.slopes ? a.slopes[head] : 0.f;
-    for (uint32_t j = lo; j < hi; j++) {
+    for (uint32_t j0 = lo; j0 < hi; j0 += 32) {
+        const uint32_t j = j0 + lane, n = min(32u, hi - j0);
         bool ok;
-        const size_t at = page_row(c, table, j, head / c.group, &ok) + lane * E;
+        const size_t at = page_row(c, table, min(j, hi - 1), head / c.group, &ok);
+        const uint4* const kp = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(c.k) + at);
         float t = 0.f;
+#pragma unroll 4
+        for (uint32_t d = 0; d < HD / 8; d++) {
+            const uint4 x = qp[d], y = kp[d];
 #pragma unroll
-        for (uint32_t e = 0; e < E; e++) t = fmaf(x[e], to_f32(reinterpret_cast<const T*>(c.k)[at + e]), t);
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
+            for (uint32_t e = 0; e < 4; e++) {
+                const float2 u = Half2<T>::unpack(reinterpret_cast<const uint32_t*>(&x)[e]), v = Half2<T>::unpack(reinterpret_cast<const uint32_t*>(&y)[e]);
+                t = fmaf(u.x, v.x, t);
+                t = fmaf(u.y, v.y, t);
+            }
+        }
         t *= a.scale;
         if (a.cap != 0.f) t = a.cap * tanhf(t / a.cap);
-        t = (t - slope * (float)(pos - (int32_t)j)) * kLog2e;
-        const float top = fmaxf(m, t), old = top == -INFINITY ? 1.f : exp2_approx(m - top), p = exp2_approx(top == -INFINITY ? t : t - top);
-        l = fmaf(l, old, p);
+        t = lane < n ? (t - slope * (float)(pos - (int32_t)j)) * kLog2e : -INFINITY;
+        float top = fmaxf(m, t);
 #pragma unroll
-        for (uint32_t e = 0; e < E; e++) o[e] = fmaf(o[e], old, p * to_f32(reinterpret_cast<const T*>(c.v)[at + e]));
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const float old = top == -INFINITY ? 1.f : exp2_approx(m - top), p = exp2_approx(top == -INFINITY ? t : t - top);
+        float sum = p;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        l = fmaf(l, old, sum);
+#pragma unroll
+        for (uint32_t e = 0; e < E; e++) o[e] *= old;
+#pragma unroll 4
+        for (uint32_t i = 0; i < n; i++) {
+            const float w = __shfl_sync(0xffffffffu, p, i);
+            const T* const vp = reinterpret_cast<const T*>(c.v) + __shfl_sync(0xffffffffu, at, i) + lane * E;
+#pragma unroll
+            for (uint32_t e = 0; e < E; e++) o[e] = fmaf(w, to_f32(vp[e]), o[e]);
+        }
         m = top;
     }
 #pragma unroll
     for (uint32_t e = 0; e < E; e++) out[e] = o[e];
     return make_float2(m, l);
+}
+// The first and the last of the positions lo .. hi of a table that have a value of key head h which is no number, by a warp; {0xFFFFFFFF, 0}: none has.
+template <typename T, int HD>
+__device__ __noinline__ uint2 not_finite_values(const Cache& c, const int32_t* table, uint32_t h, uint32_t lo, uint32_t hi) {
+    constexpr uint32_t CH = HD / 8;                // 16-byte pieces of a row
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t first = 0xFFFFFFFFu, last = 0;
+#pragma unroll 4
+    for (uint32_t j = lo + lane / CH; j < hi; j += 32 / CH) {
+        bool ok;
+        const uint4 x = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(c.v) + page_row(c, table, j, h, &ok))[lane % CH];
+        if (Half2<T>::not_finite(x.x) | Half2<T>::not_finite(x.y) | Half2<T>::not_finite(x.z) | Half2<T>::not_finite(x.w)) {
+            first = min(first, j);
+            last = j;
+        }
+    }
+    __syncwarp();
+    return make_uint2(__reduce_min_sync(0xffffffffu, first), __reduce_max_sync(0xffffffffu, last));
 }
 
 template <typename T, int HD>
@@ -184,6 +224,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
         lo = max(c.shared, first_seen(base_pos + (int32_t)(tile * kTcRows / c.group), a.window));
         hi = (uint32_t)max(0, base_pos + (int32_t)(last / c.group) + 1);
         table += (size_t)entry * c.table_ld;
+        if (tid == 0) {                        // for whoever looks for values that are no numbers, in the end
+            found[2] = lo;
+            found[3] = hi;
+        }
     }
     const bool any = entry != 0xFFFFFFFFu && tile * kTcRows < n_pairs;
     const uint32_t first_row = tile * kTcRows, start = lo & ~(w.box - 1), steps = any && hi > lo ? (hi - start + kKeys - 1) / kKeys : 0;
@@ -510,7 +554,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
                 }
             }
             if (live && ok && !w.direct) *reinterpret_cast<float2*>(pml) = make_float2(ref - kBelow, l);
+            // Rows with a result that is no number, and whether that is theirs: only if all such values lie where the row looks.  Looked for where one of these
+            // rows does not look: beside the diagonal, as a rule, not the row's own positions, which are as many as the cache has.  (1024 rows over 3000 positions, 64
+            // heads of 128, an infinite value in the middle that all rows see: 0.19 ms, 142 with all rows done again, 0.13 without it; at the last position, where
+            // only one row sees it and the rest of its tile is done again: 29 ms.)
             uint32_t again = __ballot_sync(0xffffffffu, live && ok && odd && cut);
+            if (again) {
+                const bool mine = again >> lane & 1;
+                const uint32_t from = max(found[2], start + b0 * kKeys), to = min(found[3], start + (b0 + n_blocks) * kKeys);
+                const uint32_t front = min(to, __reduce_max_sync(0xffffffffu, mine ? row_lo : 0)), behind = max(from, __reduce_min_sync(0xffffffffu, mine ? row_hi : 0xFFFFFFFFu));
+                const uint2 x = not_finite_values<T, HD>(c, table, h, from, front), y = not_finite_values<T, HD>(c, table, h, behind, to);
+                again = __ballot_sync(0xffffffffu, mine && (x.x < row_lo || (y.x <= y.y && y.y >= row_hi)));
+            }
             while (again) {
                 const uint32_t from = __ffs(again) - 1;
                 again &= again - 1;
