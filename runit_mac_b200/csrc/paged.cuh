@@ -29,6 +29,13 @@ struct Cache {
 __device__ __forceinline__ void report(const Cache& c) {
     if (c.status) atomicCAS(c.status, 0, 5);
 }
+// By every thread of a launch that reads what came before its call without having waited for the launch in front of it, which belongs to the call and has let it
+// begin behind its own wait.  So whatever came before has ended and is in the second-level cache; an acquiring load sees to it that nothing read behind it
+// comes from a copy that the SM has kept since earlier (the wait would do so, too).
+__device__ __forceinline__ void acquire_ahead(const Cache& c) {
+    int32_t first;
+    asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(first) : "l"(c.q_start) : "memory");
+}
 // Element offset of row `pos % page` of key head h in the page of position pos; table: the sequence's pages.  A page outside the pool is
 // reported and page 0 taken instead, for whoever only reads; *ok says so.
 __device__ __forceinline__ size_t page_row(const Cache& c, const int32_t* table, uint32_t pos, uint32_t h, bool* ok) {

@@ -600,8 +600,8 @@ __global__ void __launch_bounds__((WIDE ? kWideWarps : kMergeWarps) * 32) merge_
     const Cache& c = a.c;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint64_t pairs = (uint64_t)c.rows * c.heads, orow = WIDE ? blockIdx.x : (uint64_t)blockIdx.x * kMergeWarps + warp;
-    // What came before the launches of this call was over before any of them began: the lengths are read ahead of the wait, which every warp does all the same, as
-    // whoever comes next relies on this launch's being the last to end.
+    // The lengths are read ahead of the wait, which every warp does all the same, as whoever comes next relies on this launch's being the last to end.
+    acquire_ahead(c);
     const uint32_t token = (uint32_t)(orow / c.heads), head = (uint32_t)(orow % c.heads);
     const uint32_t s = orow < pairs ? sequence_by_warp(c, token) : c.n_seqs;
     const Seq q = s < c.n_seqs ? sequence(c, s) : Seq{0, 0, 0};

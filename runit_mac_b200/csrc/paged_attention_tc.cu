@@ -137,7 +137,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = tmem_holder;
-    if (!w.beside) grid_dependency_wait();
+    if (w.beside) {
+        acquire_ahead(c);
+        asm volatile("fence.proxy.async.global;" ::: "memory");  // for the pages, which the copies read
+    } else grid_dependency_wait();
     grid_launch_dependents();
 
     // which rows and positions
