@@ -55,11 +55,11 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory"); }
-// What differs between the two 16-bit types: products, packing, bits that are no number, and their range.  Weights 2^(s - ref) are rounded to the type with ref
-// kLift below the row's largest score (the kernel for many rows: kLift - kRise, and a score may exceed ref + that by kRise before ref follows).  f16 has ten bits
-// down to 2^-14 only and nothing below 2^-25: with the largest weights at 2^15, those down to 2^-29 of the largest (2^-25 in the other kernel) are rounded by half a step
-// relative to themselves, and 131072 weights below that, 2^-8 of the sum at most, by 2^-19 of it together.  With the largest at 1 a row whose best key is 17 nats ahead of
-// thousands of others lost up to all that those others have.  bf16 has its eight bits throughout.
+// What differs between the two 16-bit types: products, packing, bits that are no number, and their range.  Weights are 2^(s - ref) when they are rounded to the
+// type, ref kLift below a row's largest score; in the kernel for many rows kLift - kRise below the one that was the largest when ref was set last, which scores may
+// exceed by kRise.  f16 has ten bits down to 2^-14 only and nothing below 2^-25: with the largest weights at 2^15, those down to 2^-29 of the largest (2^-25 in the
+// other kernel) are off by half a step relative to themselves, and 131072 weights below that, 2^-8 of the sum at most, by 2^-19 of it together.  (With the largest
+// at 1, a row whose best key is 17 nats ahead of thousands of others lost up to all that the others have.)  bf16 has its eight bits throughout.
 template <typename T> struct Half2;
 template <> struct Half2<__half> {
     static constexpr float kLift = 15.f, kRise = 4.f;
