@@ -2,8 +2,8 @@
 //
 // With m = max x, d = x - m, Z = sum e^d: log p = d - log Z, entropy = log Z - (sum e^d d) / Z.  The maximal entry's own 1 is kept out of the sum, Z = 1 + z
 // and log Z = log1p(z): when that entry holds nearly all of the mass, its log probability and the entropy are tiny and keep their digits.
-// Bound: HBM and the issue slots, close to each other: 2048 rows of 152064 bf16 logits with 5 alternatives take 122 us, 5.1 TB/s.  Few rows: latency; 8 rows of
-// 151936 with 20 alternatives, a cluster of 16 blocks for each, 13.0 us.
+// Bound: HBM and the issue slots, close to each other: 2048 rows of 152064 bf16 logits with 5 alternatives take 123 to 130 us, 5.1 to 4.8 TB/s (two
+// GPUs).  Few rows: latency; 8 rows of 151936 with 20 alternatives, a cluster of 16 blocks for each, 13.2 us.
 #include "gemv_common.cuh"
 #include "paged.cuh"
 #include "tcgen05.cuh"
@@ -628,7 +628,7 @@ template <typename T, bool TOP, uint32_t ADDERS> static int32_t launch(runit_ctx
     return runit_after_launch(ctx, "token_logprobs");
 }
 // A second warp to add up where blocks have rows one behind the other and short ones, so that the alternatives take as long as the reading (4000 rows of 2000, 20
-// alternatives: 64 us with one, 45 with two; 2048 rows of 152064 with 5: 119 and 122).
+// alternatives: 64 us with one, 45 with two; 2048 rows of 152064 with 5: 119 and 122, both on one GPU).
 template <typename T, bool TOP> static int32_t run(runit_ctx* ctx, const Args& a) {
     if constexpr (TOP)
         if (a.rows > (uint32_t)ctx->sm_count * kBlocksPerSm && a.n < 32768) return launch<T, TOP, 2>(ctx, a);
