@@ -204,7 +204,7 @@ int32_t runit_flush(runit_ctx_t* ctx) {
         const int32_t why = ctx->h_status[0];
         ctx->h_status[0] = 0;
         // barriers wait again after this report; the tickets of a launch that gave up are cleared ahead of whatever the stream gets next
-        cudaError_t c = ctx->d_abort ? cudaMemsetAsync(ctx->d_abort, 0, 4, ctx->stream) : cudaSuccess;
+        cudaError_t c = ctx->d_abort ? cudaMemsetAsync(ctx->d_abort, 0, 64, ctx->stream) : cudaSuccess;
         if (c == cudaSuccess && ctx->d_tc) c = cudaMemsetAsync(ctx->d_tc, 0, runit::tcg::kTicketBytes, ctx->stream);
         if (c != cudaSuccess) runit_fail(ctx, RUNIT_ERR_LAUNCH, "clearing after a wait that gave up: %s", cudaGetErrorString(c));
         if (why == 4) {

@@ -66,6 +66,7 @@ struct runit_ctx {
     int32_t* d_status = nullptr;        // device address of the status word written by kernels with bounded waits
     int32_t* h_status = nullptr;        // the same word, host side (pinned, mapped)
     uint32_t* d_abort = nullptr;        // device word: set by the first peer barrier that gave up; later barriers skip their wait
+                                        // word 8: a paged operator has set the status; the flush that reports it clears all of them
     void* d_am = nullptr;               // greedy epilogue of the GEMV: ticket word at 0, result pair at 16, per-tile pairs from 256
     uint32_t* d_xq_ctl = nullptr;       // batched GEMV with the pre-pass inside: launch number, exit tickets, one flag per unit (from word 64)
     void* d_kq = nullptr;               // Q6_K GEMV with K split over CTAs: 2048 tile tickets (zero at rest), then 1 MiB of partial sums

@@ -1,5 +1,6 @@
 """Starts, lengths and pages on the device that contradict each other or the tensors: what is reported, and what is left as it was."""
 import ctypes as C
+import time
 
 import numpy as np
 import pytest
@@ -83,3 +84,45 @@ def test_an_append_at_shared_positions_goes_to_the_pages_of_the_first_sequence(c
     np.testing.assert_array_equal(k, want_k)
     np.testing.assert_array_equal(v, want_v)
     np.testing.assert_array_equal(q, x[:, :2])
+
+
+@pytest.mark.parametrize("what", ["pages", "lengths"])
+@pytest.mark.parametrize("op", ["append", "single rows", "a prompt"])
+def test_many_contradictions_take_no_longer_than_one(ctx, op, what):
+    """Every page (or length) bad, call after call: each flush reports it, and no call takes a hundred times what a good one does."""
+    import runit_mac_b200 as R
+    n_seqs, rows, heads, length = {"append": (4, 1000, 8, 4000), "single rows": (16, 1, 8, 8000), "a prompt": (2, 300, 8, 6000)}[op]
+    page, dim, ld = 16, 64, 500
+    pool, table = ctx.buffer_from(np.zeros(heads * page * dim, np.uint16)), ctx.buffer_from(np.zeros((n_seqs, ld), np.int32))
+    starts, lens = ctx.buffer_from(np.arange(n_seqs + 1, dtype=np.int32) * rows), ctx.buffer_from(np.full(n_seqs, length, np.int32))
+    cfg = R.PagedCfg(heads=heads, kv_heads=heads, dim=dim, page=page, n_pages=1, type=R.TYPE_F16, window=0, scale=0.125, cap=0.0, slopes=None, k_pages=pool.ptr, v_pages=pool.ptr)
+    batch = R.PagedBatch(n_seqs=n_seqs, rows=n_seqs * rows, table_ld=ld, shared_len=0, table=table.ptr, q_start=starts.ptr, kv_len=lens.ptr)
+    n, width = R.paged_attention_scratch_bytes(ctx, cfg, batch), heads * dim
+    proj, q, out, scratch = ctx.buffer_from(np.zeros((n_seqs * rows, 3 * width), np.uint16)), ctx.buffer_from(np.zeros((n_seqs * rows, width), np.uint16)), ctx.new_buffer(n_seqs * rows * width * 2), ctx.new_buffer(n)
+
+    def timed(bad):
+        took = []
+        for _ in range(4):
+            t = time.perf_counter()
+            if op == "append":
+                R.paged_append(ctx, C.byref(cfg), C.byref(batch), proj, R.TYPE_F16, 3 * width, None, 0, q, width)
+            else:
+                R.paged_attention(ctx, C.byref(cfg), C.byref(batch), q, width, out, width, scratch, n)
+            if bad:
+                with pytest.raises(R.KernelError) as e:
+                    ctx.flush()
+                assert e.value.status == 2
+            else:
+                ctx.flush()
+            took.append(time.perf_counter() - t)
+        return min(took)
+
+    good = timed(False)
+    if what == "pages":
+        table.upload(np.full((n_seqs, ld), -7, np.int32))
+    else:
+        lens.upload(np.full(n_seqs, ld * page + 1, np.int32))
+    assert timed(True) <= 20 * good + 2e-3
+    table.upload(np.zeros((n_seqs, ld), np.int32))
+    lens.upload(np.full(n_seqs, length, np.int32))
+    timed(False)
