@@ -59,7 +59,8 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volat
 // type, ref kLift below a row's largest score; in the kernel for many rows kLift - kRise below the one that was the largest when ref was set last, which scores may
 // exceed by kRise.  f16 has ten bits down to 2^-14 only and nothing below 2^-25: with the largest weights at 2^15, those down to 2^-29 of the largest (2^-25 in the
 // other kernel) are off by half a step relative to themselves, and 131072 weights below that, 2^-8 of the sum at most, by 2^-19 of it together.  (With the largest
-// at 1, a row whose best key is 17 nats ahead of thousands of others lost up to all that the others have.)  bf16 has its eight bits throughout.
+// at 1, a row whose best key is 17 nats ahead of thousands of others lost up to all that the others have.)  bf16 has its eight bits throughout, and values up to the
+// end of f32's range: no weight exceeds 1.
 template <typename T> struct Half2;
 template <> struct Half2<__half> {
     static constexpr float kLift = 15.f, kRise = 4.f;

@@ -111,7 +111,7 @@ __device__ __noinline__ uint2 not_finite_values(const Cache& c, const int32_t* t
 template <typename T, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const AttnArgs a, const TcArgs w) {
     using S = TcShape<HD>;
-    constexpr float kRise = Half2<T>::kRise, kBelow = Half2<T>::kLift > kRise ? Half2<T>::kLift - kRise : 0.f;       // what weights are relative to: ref - kBelow
+    constexpr float kRise = Half2<T>::kRise, kBelow = Half2<T>::kLift - kRise;       // weights are relative to ref - kBelow
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[2 * S::kSlots + 14];
     __shared__ uint32_t tmem_holder, found[4], sums[kTcThreads / 32];

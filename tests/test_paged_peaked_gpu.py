@@ -43,3 +43,13 @@ def test_a_key_far_ahead_of_the_others(ctx, name, lead, kind):
     """The bound is that of every batch: a weight is off by half a step of the cache's type relative to its own size, also those e^-17 below the largest."""
     b = _peaked(kind=kind, lead=lead, **PEAKED[name])
     check(b, b.attend(ctx), name)
+
+
+@pytest.mark.parametrize("rows,n_seqs,shared", [(1, 40, 0), (200, 1, 0), (1, 300, 512)])
+@pytest.mark.parametrize("late", [3.0, 5.0, 5.5])
+def test_values_near_the_end_of_the_range(ctx, rows, n_seqs, shared, late):
+    """A key somewhat ahead of those in front of it, with values of which e^late do not fit f32: its weight is 1 of the sum, whatever it is before that is divided by."""
+    b = _peaked(n_seqs, rows, 700, 16, 4, 64, "bf16", late, shared=shared, at=150)
+    b.v[b.table[0, :-(-700 // 16)]] = 0.0
+    b.v[b.table[0, 150 // 16], :, 150 % 16] = rounded(np.full((4, 64), 2.9e38 / np.exp(late) * 2.5), "bf16")
+    check(b, b.attend(ctx))
