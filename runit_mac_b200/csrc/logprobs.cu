@@ -2,8 +2,8 @@
 //
 // With m = max x, d = x - m, Z = sum e^d: log p = d - log Z, entropy = log Z - (sum e^d d) / Z.  The maximal entry's own 1 is kept out of the sum, Z = 1 + z
 // and log Z = log1p(z): when that entry holds nearly all of the mass, its log probability and the entropy are tiny and keep their digits.
-// Bound: HBM and the issue slots, close to each other: 2048 rows of 152064 bf16 logits with 5 alternatives take 123 to 130 us, 5.1 to 4.8 TB/s (two
-// GPUs).  Few rows: latency; 8 rows of 151936 with 20 alternatives, a cluster of 16 blocks for each, 13.2 us.
+// Bound: HBM and the issue slots, close to each other: 2048 rows of 152064 bf16 logits with 5 alternatives take 123 to 131 us, 5.1 to 4.8 TB/s
+// (three GPUs).  Few rows: latency; 8 rows of 151936 with 20 alternatives, a cluster of 16 blocks for each, 13.2 us.
 #include "gemv_common.cuh"
 #include "paged.cuh"
 #include "tcgen05.cuh"

@@ -3,7 +3,7 @@
 // y_i = x_i cos a_i - x_{i+h} sin a_i, y_{i+h} = x_i sin a_i + x_{i+h} cos a_i for i < h = rot_dims / 2, a_i = position * freq_i.  The position is an
 // integer and freq_i the sum of two floats, so that the angle of a far position keeps its 24 bits (a product of two floats loses as many as the
 // position has); from 2^17 on it is formed in 64 bits.  One rounding, at the end.
-// Bound: HBM (every value is read once and written once: 7167 rows of 16 + 32 heads of 128 from f32, 264 MB, in 45 us; a block per row of 192 threads that ask for
+// Bound: HBM (every value is read once and written once: 7167 rows of 16 + 32 heads of 128 from f32, 264 MB, in 45 to 46 us; a block per row of 192 threads that ask for
 // their 128 bytes each before anything else; 128 threads with 4 such pieces 3 more); latency for a few rows.
 #include "linear_state.cuh"
 #include "paged.cuh"

@@ -9,7 +9,7 @@
 // Tensor memory, 512 columns: S 64 and P 2 x 32 of each tile, O 128 of each.
 // Bound: products of 64 positions, whose operands from shared memory take 48 clocks instead of 32 (1260 a half for both tiles), and the warps of the softmax, which
 // have 512 clocks of exponentials a half and some 1200 with all the rest, two of them a scheduler.  3584 (row, head) pairs over 32768 positions, dim 128:
-// 71 us, 850 TFLOP/s; prompts of 3 x 700 .. 2048 rows behind 2048 .. 4096 positions, 16 heads of 128, scores capped, 115 us, 540 TFLOP/s (256
+// 71 us, 850 TFLOP/s; prompts of 3 x 700 .. 2048 rows behind 2048 .. 4096 positions, 16 heads of 128, scores capped, 115 to 118 us, 540 to 526 TFLOP/s (256
 // tiles leave 148 SMs idle for a fifth of that: 38 blocks on the busiest, 30.8 on average).  Whole blocks of 128 positions at a time: 5% slower.
 // K and V of a block come by TMA as boxes of whole pages or of 128 positions; positions outside of what the CTA's rows see are zeros in V.
 #include "paged_attention.cuh"
